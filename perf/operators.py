@@ -133,7 +133,7 @@ def work(case):
 # ---- inputs -----------------------------------------------------------------------------
 def _power_of_two(top):
     """The smallest power of two s >= 2^-118 with top <= 448 s."""
-    mantissa, exponent = torch.frexp(top)
+    mantissa, exponent = torch.frexp(top.clamp_min(2.0 ** -120))
     return torch.ldexp(torch.ones_like(top), (exponent - 9 + (mantissa > 0.875)).clamp(-118, 120))
 
 
