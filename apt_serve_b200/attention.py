@@ -148,11 +148,16 @@ def paged_decode_attention(query: torch.Tensor, key_cache: torch.Tensor,
                            value_cache: torch.Tensor, block_tables: torch.Tensor,
                            seq_lens: torch.Tensor, scale: float,
                            out: Optional[torch.Tensor] = None,
-                           workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+                           workspace: Optional[torch.Tensor] = None, k_scale: Optional[torch.Tensor] = None,
+                           v_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Decode attention over K/V blocks: ``query [B, H*D]``, caches
     ``[NB, BS, H, D]``, ``block_tables`` int32 ``[B, max_blocks]``, ``seq_lens``
     int32 ``[B]`` -> ``[B, H*D]`` (the ``flash_attn_with_kvcache`` call of
-    aptserve_flash_attn.py:452-461)."""
+    aptserve_flash_attn.py:452-461).  With ``k_scale`` / ``v_scale`` (fp32 ``[NB, H]``) the caches are 8-bit ones
+    (``ops.reshape_and_cache_flash``), the query of any type."""
+    if k_scale is not None or v_scale is not None or key_cache.dtype in (torch.float8_e4m3fn, torch.uint8):
+        return _attend_fp8("paged_decode_attention", query, key_cache, value_cache, block_tables, None, seq_lens, 1, scale,
+                           k_scale, v_scale, out, workspace)
     dev = N.require_cuda(query, key_cache, value_cache, block_tables, seq_lens)
     b = query.shape[0]
     _, bs, h, d = key_cache.shape
@@ -174,6 +179,60 @@ def paged_decode_attention(query: torch.Tensor, key_cache: torch.Tensor,
             b, bt.shape[1], h, d, bs, query.stride(0), out.stride(0), key_cache.stride(0),
             float(scale), N.ptr(workspace), workspace.numel(), N.dtype_enum(query),
             N.current_stream(dev)))
+    return out
+
+
+def paged_prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, block_tables: torch.Tensor,
+                           query_start_loc: torch.Tensor, seq_lens: torch.Tensor, max_query_len: int, scale: float,
+                           k_scale: torch.Tensor, v_scale: torch.Tensor, out: Optional[torch.Tensor] = None,
+                           workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of several new tokens per request over its whole context in an 8-bit cache, the new tokens' own rows included (a chunk of
+    a prompt behind a cached prefix, drafted tokens to be verified): rows ``query_start_loc[r] ... query_start_loc[r + 1]`` (int32
+    ``[B + 1]``, at most ``max_query_len`` each) of ``query [T, H*D]`` are the last of request ``r``'s ``seq_lens[r]`` tokens, each
+    attends to the tokens up to itself -> ``[T, H*D]``.  Rows that belong to no request are left as they are in ``out``."""
+    return _attend_fp8("paged_prefix_attention", query, key_cache, value_cache, block_tables, query_start_loc, seq_lens, max_query_len,
+                       scale, k_scale, v_scale, out, workspace)
+
+
+def _attend_fp8(op, query, key_cache, value_cache, block_tables, starts, seq_lens, max_rows, scale, k_scale, v_scale, out, workspace):
+    ops.check_fp8_cache(op, key_cache, value_cache, k_scale, v_scale)
+    dev = N.require_cuda(query, key_cache, value_cache, block_tables, starts, seq_lens, k_scale, v_scale, out, workspace)
+    nb, bs, h, d = key_cache.shape
+    if query.dim() != 2 or query.shape[1] != h * d or query.stride(1) != 1:
+        raise RuntimeError(f"{op}: query must be [T, {h * d}] with contiguous rows")
+    t = query.shape[0]
+    if out is None:
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    elif out.shape != query.shape or out.dtype != query.dtype or out.stride(1) != 1:
+        raise RuntimeError(f"{op}: out must be like query, with contiguous rows")
+    bt = _i32(block_tables, "block_tables")
+    sl = _i32(seq_lens, "seq_lens")
+    if bt.dim() != 2 or sl.dim() != 1:
+        raise RuntimeError(f"{op}: block_tables must be [B, max_blocks], seq_lens [B]")
+    if starts is None:
+        b = t
+    else:
+        starts = _i32(starts, "query_start_loc")
+        if starts.dim() != 1 or starts.shape[0] < 1 or max_rows < 0:
+            raise RuntimeError(f"{op}: query_start_loc must hold a start for every request and the end, max_query_len must not be negative")
+        b = starts.shape[0] - 1
+    if bt.shape[0] < b or sl.shape[0] < b:
+        raise RuntimeError(f"{op}: {bt.shape[0]} block tables and {sl.shape[0]} lengths for {b} requests")
+    if t == 0 or b == 0:
+        return out
+    if bt.shape[1] == 0:
+        raise RuntimeError(f"{op}: block_tables without columns")
+    lib = N.lib()
+    with N.on_device(dev):
+        if workspace is None:
+            workspace, ws_bytes = _scratch_of(dev, lib.aps_kv8_attention_workspace_bytes(t, bt.shape[1], bs, h, d))
+        else:
+            ws_bytes = workspace.numel() * workspace.element_size()
+        N.check(lib.aps_kv8_attention(
+            out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+            bt.data_ptr(), N.ptr(starts), sl.data_ptr(), b, t, max_rows, bt.shape[1], h, d, bs, nb,
+            query.stride(0) if t > 1 else h * d, out.stride(0) if t > 1 else h * d, key_cache.stride(0), k_scale.stride(0), float(scale),
+            workspace.data_ptr(), ws_bytes, N.dtype_enum(query), N.current_stream(dev)))
     return out
 
 
@@ -686,17 +745,23 @@ class FlashAttentionImpl:
         if head_size not in supported:
             raise ValueError(f"Head size {head_size} is not supported by FlashAttention. "
                              f"Supported head sizes are: {supported}.")
+        self.fp8_cache = kv_cache_dtype in ops.FP8_CACHE
 
     # -- reference op sequence ------------------------------------------------- #
     def forward(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
                 kv_cache: Optional[torch.Tensor], shared_cache: Optional[torch.Tensor],
-                attn_metadata: FlashAttentionMetadata, kv_scale: float = 1.0) -> torch.Tensor:
+                attn_metadata: FlashAttentionMetadata, kv_scale=1.0) -> torch.Tensor:
         """``query [T, H*D]``; ``key`` / ``value`` ``[T or N_tot, H*D]``;
         ``kv_cache [2, NB, BS, H, D]``; ``shared_cache [2, 2NB, BS, H, D]``
         -> ``[T, H*D]``.  Follows the reference step by step: which cache-write op
         runs (aptserve_flash_attn.py:331-387), var-len attention for prompts
-        (:405-447), paged attention for decode tokens (:449-475)."""
-        assert kv_scale == 1.0, "kv_scale is not supported in FlashAttention."
+        (:405-447), paged attention for decode tokens (:449-475).
+
+        With an 8-bit cache (``kv_cache_dtype="fp8"``) ``kv_cache`` holds e4m3 numbers and ``kv_scale`` is the tensor of their scales,
+        fp32 ``[2, NB, H]``, which the writes set (``ops.reshape_and_cache_flash``); hidden-cached requests are refused."""
+        if self.fp8_cache:
+            return self._forward_fp8(query, key, value, kv_cache, attn_metadata, kv_scale)
+        assert not isinstance(kv_scale, torch.Tensor) and kv_scale == 1.0, "kv_scale is not supported in FlashAttention."
         if attn_metadata.num_prefill_tokens == 0 and attn_metadata.num_hidden_cache_tokens == 0:
             output = self._plain_decode(query, key, value, kv_cache, attn_metadata)
             if output is not None:
@@ -766,6 +831,37 @@ class FlashAttentionImpl:
             paged_decode_attention(q2, kc, vc, decode_meta.block_tables,
                                    decode_meta.seq_lens_tensor, self.scale, out=o2)
         return output.reshape(num_tokens, hidden_size)
+
+    def _forward_fp8(self, query, key, value, kv_cache, m, kv_scale) -> torch.Tensor:
+        """``forward`` over an 8-bit cache: prompts without a cached prefix attend to their own rows as they are, everything else to what
+        the cache holds, the step's own rows included."""
+        if m.num_hidden_cache_tokens != 0:
+            raise ValueError("hidden-cached requests need a 16-bit or fp32 cache: hidden rows are not held in 8 bits")
+        num_tokens, hidden_size = query.shape
+        n_prefill, n_decode = m.num_prefill_tokens, m.num_decode_tokens
+        query = query.reshape(-1, self.num_heads * self.head_size)
+        key = key.reshape(-1, self.num_kv_heads, self.head_size)
+        value = value.reshape(-1, self.num_kv_heads, self.head_size)
+        assert key.shape[0] == value.shape[0] == query.shape[0] == n_prefill + n_decode
+        if kv_cache is not None:
+            if not isinstance(kv_scale, torch.Tensor) or kv_scale.dim() != 3 or kv_scale.shape[0] < 2:
+                raise ValueError("an 8-bit cache needs kv_scale, the [2, blocks, heads] tensor of its scales")
+            key_cache, value_cache, k_scale, v_scale = kv_cache[0], kv_cache[1], kv_scale[0], kv_scale[1]
+            ops.reshape_and_cache_flash(key, value, key_cache, value_cache, m.slot_mapping, self.kv_cache_dtype, k_scale, v_scale)
+        output = torch.empty_like(query, memory_format=torch.contiguous_format)
+        if (prefill_meta := m.prefill_metadata) is not None:
+            if kv_cache is None or prefill_meta.block_tables is None or prefill_meta.block_tables.numel() == 0:
+                output[:n_prefill] = _varlen_prefill_attention(
+                    query[:n_prefill].view(-1, self.num_heads, self.head_size), key[:n_prefill], value[:n_prefill],
+                    prefill_meta.seq_start_loc, prefill_meta.max_prefill_seq_len, self.scale).reshape(n_prefill, -1)
+            else:
+                paged_prefix_attention(query[:n_prefill], key_cache, value_cache, prefill_meta.block_tables, prefill_meta.query_start_loc,
+                                       prefill_meta.seq_lens_tensor, prefill_meta.max_query_len, self.scale, k_scale, v_scale,
+                                       out=output[:n_prefill])
+        if (decode_meta := m.decode_metadata) is not None:
+            paged_decode_attention(query[n_prefill:], key_cache, value_cache, decode_meta.block_tables, decode_meta.seq_lens_tensor,
+                                   self.scale, out=output[n_prefill:], k_scale=k_scale, v_scale=v_scale)
+        return output.view(num_tokens, hidden_size)
 
     def _plain_decode(self, query, key, value, kv_cache, m) -> Optional[torch.Tensor]:
         """``forward`` for what almost every step of plain serving is, a batch of decode tokens without hidden-cached
@@ -843,9 +939,10 @@ class Attention(torch.nn.Module):
                                        alibi_slopes, sliding_window, kv_cache_dtype,
                                        blocksparse_params)
 
-    def forward(self, query, key, value, kv_cache, shared_cache, attn_metadata) -> torch.Tensor:
+    def forward(self, query, key, value, kv_cache, shared_cache, attn_metadata, kv_scale=None) -> torch.Tensor:
+        """``kv_scale``: the scales ``[2, NB, H]`` of an 8-bit cache."""
         return self.impl.forward(query, key, value, kv_cache, shared_cache, attn_metadata,
-                                 self._kv_scale)
+                                 self._kv_scale if kv_scale is None else kv_scale)
 
     def extra_repr(self) -> str:
         return (f"head_size={self.impl.head_size}, num_heads={self.impl.num_heads}, "

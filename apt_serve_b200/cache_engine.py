@@ -16,6 +16,10 @@ so each layer gets a dedicated ``[2, NB, BS, 1, E]`` hidden cache with the same 
 numbering.  Block moves address PHYSICAL blocks, both planes at once, so a swap or a copy
 of physical block ``p`` carries the hidden blocks ``p`` and ``p + NB`` with it;
 ``physical_block_map`` folds a map written in logical ids.
+
+``dtype=torch.float8_e4m3fn`` gives 8-bit K/V caches: each layer has a tensor of scales ``[2, NB, H]`` beside its cache
+(``gpu_scale``, ``cpu_scale``; ``ops.reshape_and_cache_flash``), which moves with the blocks.  Hidden rows are not held in 8 bits:
+there is no hidden cache then.
 """
 from __future__ import annotations
 
@@ -67,12 +71,20 @@ class CacheEngine:
         self.device = torch.device(device)
         if pin_memory is None:
             pin_memory = torch.cuda.is_available()
+        self.fp8 = dtype == torch.float8_e4m3fn
+        if self.fp8 and with_shared_cache:
+            raise ValueError("the shared cache holds re-projected hidden rows, which an 8-bit cache does not have")
         self.gpu_cache = self._allocate(num_gpu_blocks, self.device, False)
         self.cpu_cache = self._allocate(num_cpu_blocks, torch.device("cpu"), pin_memory)
         # hidden rows of a layer: its K/V planes when they are as wide as a hidden row,
         # else a dedicated tensor with the same [2, NB, BS] slot numbering
-        self.aliased_hidden = self.hidden_size == num_kv_heads * head_size
-        if self.aliased_hidden:
+        self.aliased_hidden = self.hidden_size == num_kv_heads * head_size and not self.fp8
+        self.gpu_scale = self.cpu_scale = None
+        if self.fp8:
+            self.gpu_hidden_cache = self.cpu_hidden_cache = None
+            self.gpu_scale = self._allocate_scales(num_gpu_blocks, self.device, False)
+            self.cpu_scale = self._allocate_scales(num_cpu_blocks, torch.device("cpu"), pin_memory)
+        elif self.aliased_hidden:
             self.gpu_hidden_cache, self.cpu_hidden_cache = self.gpu_cache, self.cpu_cache
         else:
             self.gpu_hidden_cache = self._allocate(num_gpu_blocks, self.device, False, hidden=True)
@@ -96,13 +108,19 @@ class CacheEngine:
                             pin_memory=bool(pin) and device.type == "cpu")
                 for _ in range(self.num_layers)]
 
+    def _allocate_scales(self, num_blocks, device, pin) -> List[torch.Tensor]:
+        return [torch.zeros((2, num_blocks, self.num_kv_heads), dtype=torch.float32, device=device,
+                            pin_memory=bool(pin) and device.type == "cpu") for _ in range(self.num_layers)]
+
     @staticmethod
     def get_cache_block_size(num_layers: int, num_kv_heads: int, head_size: int, block_size: int,
                              dtype: torch.dtype, hidden_size: Optional[int] = None) -> int:
         """Bytes of one physical block over all layers (aptserve_cache_engine.py:101-119),
-        plus the dedicated hidden rows when the planes cannot hold them."""
+        plus the dedicated hidden rows when the planes cannot hold them, or an 8-bit block's scales."""
         es = torch.empty((), dtype=dtype).element_size()
         per_layer = 2 * block_size * num_kv_heads * head_size
+        if dtype == torch.float8_e4m3fn:
+            return num_layers * (per_layer + 2 * 4 * num_kv_heads)
         if hidden_size is not None and hidden_size != num_kv_heads * head_size:
             per_layer += 2 * block_size * hidden_size
         return es * num_layers * per_layer
@@ -122,24 +140,30 @@ class CacheEngine:
         return int(budget_bytes // per_block)
 
     # ---- block moves ----------------------------------------------------------------
-    def _swap(self, src, dst, src_hidden, dst_hidden, src_to_dst: torch.Tensor) -> None:
+    def _swap(self, src, dst, src_more, dst_more, src_to_dst: torch.Tensor) -> None:
+        """``src_more`` / ``dst_more``: what moves with the blocks, dedicated hidden rows or an 8-bit cache's scales."""
         for i in range(self.num_layers):
             for plane in (0, 1):                                   # K then V (aptserve_flash_attn.py:50-56)
                 ops.swap_blocks(src[i][plane], dst[i][plane], src_to_dst)
                 if not self.aliased_hidden:
-                    ops.swap_blocks(src_hidden[i][plane], dst_hidden[i][plane], src_to_dst)
+                    ops.swap_blocks(src_more[i][plane], dst_more[i][plane], src_to_dst)
+
+    def _more(self):
+        return (self.gpu_scale, self.cpu_scale) if self.fp8 else (self.gpu_hidden_cache, self.cpu_hidden_cache)
 
     def swap_in(self, src_to_dst: torch.Tensor) -> None:
         """CPU -> GPU, physical block ids (aptserve_cache_engine.py:88-91)."""
-        self._swap(self.cpu_cache, self.gpu_cache, self.cpu_hidden_cache, self.gpu_hidden_cache, src_to_dst)
+        gpu, cpu = self._more()
+        self._swap(self.cpu_cache, self.gpu_cache, cpu, gpu, src_to_dst)
 
     def swap_out(self, src_to_dst: torch.Tensor) -> None:
         """GPU -> CPU, physical block ids (aptserve_cache_engine.py:93-96)."""
-        self._swap(self.gpu_cache, self.cpu_cache, self.gpu_hidden_cache, self.cpu_hidden_cache, src_to_dst)
+        gpu, cpu = self._more()
+        self._swap(self.gpu_cache, self.cpu_cache, gpu, cpu, src_to_dst)
 
     def copy(self, src_to_dsts: torch.Tensor) -> None:
         """Copy-on-write block copies in every layer (aptserve_cache_engine.py:98-99)."""
         ops.copy_blocks([c[0] for c in self.gpu_cache], [c[1] for c in self.gpu_cache], src_to_dsts)
         if not self.aliased_hidden:
-            ops.copy_blocks([c[0] for c in self.gpu_hidden_cache], [c[1] for c in self.gpu_hidden_cache],
-                            src_to_dsts)
+            more, _ = self._more()
+            ops.copy_blocks([c[0] for c in more], [c[1] for c in more], src_to_dsts)

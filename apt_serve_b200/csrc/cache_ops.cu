@@ -27,6 +27,7 @@
 // attention/backends/aptserve_flash_attn.py:58-65, 338-385.
 
 #include "attention_common.cuh"   // read_metadata_status, read_prefill_status
+#include "kv8_common.cuh"         // read_kv8_status
 
 #include <initializer_list>
 #include <stdlib.h>
@@ -609,7 +610,9 @@ extern "C" int aps_cache_ops_status(int* host_status, void* stream) {
   if (words[0] == 0 && words[1] != 0) APS_CUDA(cudaMemsetAsync(addr + 1, 0, sizeof(int), (cudaStream_t)stream));   // reported once
   if (*host_status != 0) return APS_OK;
   const int st = read_metadata_status(host_status, (cudaStream_t)stream);
-  return st != APS_OK || *host_status != 0 ? st : read_prefill_status(host_status, (cudaStream_t)stream);
+  if (st != APS_OK || *host_status != 0) return st;
+  const int written = read_kv8_status(host_status, (cudaStream_t)stream);
+  return written != APS_OK || *host_status != 0 ? written : read_prefill_status(host_status, (cudaStream_t)stream);
 }
 
 // Block moves between one plane of a GPU cache and one plane of the pinned CPU cache (or

@@ -1,0 +1,274 @@
+// Attention over the 8-bit cache (kv8_common.cuh), any number of query rows per request.
+//
+//   kv8_rows_kernel     CUDA-core arithmetic, one CTA per (query row, head, part of the row's tokens): every query type, head size
+//                       and block stride.  D / 16 lanes cover a row with one 16-byte load each.
+//   kv8_combine_kernel  joins the parts of rows whose tokens were cut.
+// Scores, softmax statistics and sums are fp32; a code times its scale is exact in fp32.
+#include "kv8_common.cuh"
+
+namespace aps {
+namespace {
+
+constexpr unsigned kFull = 0xffffffffu;
+constexpr int kRowWarps = 4;
+
+struct RowArgs {
+  Kv8Call c;
+  int* plan;                  // the scratch's header, as the other attention calls have it: its status is set to fine
+  float* acc; float2* ml;     // partials [row][head][split], unless splits == 1
+  int splits;
+  float scale_log2;
+};
+
+// The request of query row t, and how many tokens the row attends to (none: a zero row).  False: the row belongs to no request.
+__device__ __forceinline__ bool find_row(const Kv8Call& c, int64_t t, int& req, int& keys) {
+  if (c.starts == nullptr) {
+    req = (int)t;
+    keys = max(0, min(c.seq_lens[req], c.max_blocks * c.cache.block_size));
+    return true;
+  }
+  if (t < c.starts[0] || t >= c.starts[c.batch]) return false;
+  int lo = 0, hi = c.batch;   // starts[lo] <= t < starts[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (c.starts[mid] <= t) lo = mid; else hi = mid;
+  }
+  req = lo;
+  const int ctx = max(0, min(c.seq_lens[req], c.max_blocks * c.cache.block_size));
+  keys = max(0, ctx - c.starts[req + 1] + (int)t + 1);
+  return true;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kRowWarps * 32)
+kv8_rows_kernel(const RowArgs a) {
+  constexpr int kLanes = D / 16, kTok = 32 / kLanes, kLoads = 4;   // lanes per row, rows per load, loads at a time
+  const Kv8Call& c = a.c;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % kLanes, tsel = lane / kLanes;
+  const int64_t t = blockIdx.x / a.splits;
+  const int split = (int)(blockIdx.x % a.splits), h = blockIdx.y;
+  if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) a.plan[kPlanStatus] = kStatusOk;
+  int req, keys;
+  if (!find_row(c, t, req, keys)) return;
+  const int per = ((keys + a.splits - 1) / a.splits + 15) / 16 * 16;
+  const int begin = min(keys, split * per), end = min(keys, begin + per);
+  const int32_t* table = c.tables + (int64_t)req * c.max_blocks;
+  const int64_t row_bytes = (int64_t)c.cache.heads * D;
+
+  float q[16];
+  {
+    const T* src = static_cast<const T*>(c.query) + t * c.query_stride + (int64_t)h * D + sub * 16;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) q[i] = Elem<T>::to_float(src[i]) * a.scale_log2;
+  }
+  float acc[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  for (int t0 = begin + warp * kTok * kLoads; t0 < end; t0 += kRowWarps * kTok * kLoads) {
+    uint4 kr[kLoads], vr[kLoads];
+    float ks[kLoads], vs[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int tok = t0 + i * kTok + tsel;
+      kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
+      ks[i] = vs[i] = __int_as_float(0x7fc00000);   // a block outside the cache: the row becomes NaN
+      if (tok < end) {
+        const int64_t block = table[tok / c.cache.block_size];
+        if (block >= 0 && block < c.cache.num_blocks) {
+          const int64_t at = block * c.cache.block_stride + tok % c.cache.block_size * row_bytes + (int64_t)h * D + sub * 16;
+          kr[i] = *reinterpret_cast<const uint4*>(c.cache.key + at);
+          vr[i] = *reinterpret_cast<const uint4*>(c.cache.value + at);
+          ks[i] = c.cache.key_scale[block * c.cache.scale_stride + h];
+          vs[i] = c.cache.value_scale[block * c.cache.scale_stride + h];
+        }
+      } else {
+        vs[i] = 0.f;
+      }
+    }
+    float s[kLoads], top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      float k[16], x = 0.f;
+      e4m3x4_to_float(kr[i].x, k); e4m3x4_to_float(kr[i].y, k + 4); e4m3x4_to_float(kr[i].z, k + 8); e4m3x4_to_float(kr[i].w, k + 12);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x = fmaf(q[e], k[e], x);
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) x += __shfl_xor_sync(kFull, x, o);
+      s[i] = t0 + i * kTok + tsel < end ? x * ks[i] : -INFINITY;
+      top = fmaxf(top, s[i]);
+    }
+#pragma unroll
+    for (int o = kLanes; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+    const float now = fmaxf(m, top), ref = now == -INFINITY ? 0.f : now, down = exp2f(m - ref);
+    l *= down;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] *= down;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const float p = exp2f(s[i] - ref), w = p * vs[i];
+      l += p;
+      float v[16];
+      e4m3x4_to_float(vr[i].x, v); e4m3x4_to_float(vr[i].y, v + 4); e4m3x4_to_float(vr[i].z, v + 8); e4m3x4_to_float(vr[i].w, v + 12);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[e] = fmaf(w, v[e], acc[e]);
+    }
+    m = now;
+  }
+#pragma unroll
+  for (int o = kLanes; o < 32; o <<= 1) {
+    l += __shfl_xor_sync(kFull, l, o);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] += __shfl_xor_sync(kFull, acc[e], o);
+  }
+  // the warps' shares, in order
+  __shared__ float s_acc[kRowWarps][D];
+  __shared__ float2 s_ml[kRowWarps];
+  if (tsel == 0) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s_acc[warp][sub * 16 + e] = acc[e];
+    if (lane == 0) s_ml[warp] = make_float2(m, l);
+  }
+  __syncthreads();
+  float top = -INFINITY, sum = 0.f, w[kRowWarps];
+#pragma unroll
+  for (int i = 0; i < kRowWarps; ++i) top = fmaxf(top, s_ml[i].x);
+  const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+  for (int i = 0; i < kRowWarps; ++i) { w[i] = exp2f(s_ml[i].x - ref); sum = fmaf(w[i], s_ml[i].y, sum); }
+  const int64_t unit = (t * c.cache.heads + h) * a.splits + split;
+  for (int d = threadIdx.x; d < D; d += kRowWarps * 32) {
+    float x = 0.f;
+#pragma unroll
+    for (int i = 0; i < kRowWarps; ++i) x = fmaf(w[i], s_acc[i][d], x);
+    if (a.splits == 1)
+      static_cast<T*>(c.out)[t * c.out_stride + (int64_t)h * D + d] = Elem<T>::from_float(keys == 0 ? 0.f : x / sum);
+    else
+      a.acc[unit * D + d] = x;
+  }
+  if (a.splits > 1 && threadIdx.x == 0) a.ml[unit] = make_float2(top, sum);
+}
+
+// One warp per (query row, head).
+template <typename T>
+__global__ void __launch_bounds__(256)
+kv8_combine_kernel(const RowArgs a) {
+  const Kv8Call& c = a.c;
+  const int lane = threadIdx.x & 31, d = c.cache.head_size;
+  const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (unit >= c.rows * c.cache.heads) return;
+  const int64_t t = unit / c.cache.heads, h = unit % c.cache.heads;
+  int req, keys;
+  if (!find_row(c, t, req, keys)) return;
+  const float2* ml = a.ml + unit * a.splits;
+  const float* acc = a.acc + unit * a.splits * d;
+  float top = -INFINITY, sum = 0.f;
+  for (int i = lane; i < a.splits; i += 32) top = fmaxf(top, ml[i].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+  const float ref = top == -INFINITY ? 0.f : top;
+  for (int i = lane; i < a.splits; i += 32) sum = fmaf(exp2f(ml[i].x - ref), ml[i].y, sum);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+  T* out = static_cast<T*>(c.out) + t * c.out_stride + h * d;
+  for (int e = lane; e < d; e += 32) {
+    float x = 0.f;
+    for (int i = 0; i < a.splits; ++i) x = fmaf(exp2f(ml[i].x - ref), acc[(int64_t)i * d + e], x);
+    out[e] = Elem<T>::from_float(keys == 0 ? 0.f : x / sum);
+  }
+}
+
+// Parts a row's tokens are cut into: enough CTAs for the GPU, parts of 256 tokens at least.
+int row_splits(const Kv8Call& c) {
+  const int64_t units = c.rows * c.cache.heads, tokens = (int64_t)c.max_blocks * c.cache.block_size;
+  const int64_t want = ((int64_t)sm_count() * 8 + units - 1) / units, most = (tokens + 255) / 256;
+  const int64_t n = want < most ? want : most;
+  return (int)(n < 1 ? 1 : n > 1024 ? 1024 : n);
+}
+
+size_t row_scratch(int64_t rows, int heads, int head_size, int splits) {
+  return kPlanWords * sizeof(int) + (splits == 1 ? 0 : (size_t)rows * heads * splits * (head_size + 2) * sizeof(float));
+}
+
+template <typename T, int D>
+int launch_rows(const RowArgs& a, cudaStream_t stream) {
+  const int64_t grid = a.c.rows * a.splits;
+  APS_REQUIRE(grid < (int64_t(1) << 31), APS_ERR_SHAPE, "kv8_attention: too many rows");
+  kv8_rows_kernel<T, D><<<dim3((unsigned)grid, a.c.cache.heads), kRowWarps * 32, 0, stream>>>(a);
+  int st = launch_status("kv8_rows_kernel");
+  if (st != APS_OK || a.splits == 1) return st;
+  kv8_combine_kernel<T><<<(unsigned)((a.c.rows * a.c.cache.heads + 7) / 8), 256, 0, stream>>>(a);
+  return launch_status("kv8_combine_kernel");
+}
+
+template <typename T>
+int rows_by_head(const RowArgs& a, cudaStream_t stream) {
+  switch (a.c.cache.head_size) {
+    case 32: return launch_rows<T, 32>(a, stream);
+    case 64: return launch_rows<T, 64>(a, stream);
+    case 128: return launch_rows<T, 128>(a, stream);
+    default: return launch_rows<T, 256>(a, stream);
+  }
+}
+
+int check_call(const char* op, const Kv8Call& c) {
+  const int st = check_kv8_cache(op, c.cache, c.dtype);
+  if (st != APS_OK) return st;
+  APS_REQUIRE(c.batch >= 0 && c.rows >= 0 && c.max_blocks > 0 && c.max_rows >= 0, APS_ERR_SHAPE, "%s: bad sizes", op);
+  APS_REQUIRE((int64_t)c.max_blocks * c.cache.block_size < (int64_t(1) << 31) && c.rows < (int64_t(1) << 31), APS_ERR_SHAPE,
+              "%s: more than 2^31 tokens", op);
+  if (c.rows == 0 || c.batch == 0) return APS_OK;
+  APS_REQUIRE(c.out && c.query && c.tables && c.seq_lens && c.cache.key && c.cache.value && c.cache.key_scale && c.cache.value_scale,
+              APS_ERR_NULL_POINTER, "%s: null pointer", op);
+  const int es = dtype_size(c.dtype);
+  const int64_t row = (int64_t)c.cache.heads * c.cache.head_size;
+  APS_REQUIRE(c.query_stride >= row && c.out_stride >= row, APS_ERR_SHAPE, "%s: strides smaller than a row", op);
+  APS_REQUIRE(aligned_to(c.query, es) && aligned_to(c.out, es) && aligned_to(c.cache.key, 16) && aligned_to(c.cache.value, 16) &&
+                  c.cache.block_stride % 16 == 0 && aligned_to(c.cache.key_scale, 4) && aligned_to(c.cache.value_scale, 4) &&
+                  aligned_to(c.tables, 4) && aligned_to(c.seq_lens, 4) && aligned_to(c.starts, 4),
+              APS_ERR_MISALIGNED, "%s: the caches must be 16-byte aligned with blocks at multiples of 16 bytes", op);
+  return APS_OK;
+}
+
+}  // namespace
+}  // namespace aps
+
+using namespace aps;
+
+extern "C" size_t aps_kv8_attention_workspace_bytes(int64_t num_rows, int max_blocks_per_seq, int block_size, int num_heads, int head_size) {
+  if (num_rows <= 0 || max_blocks_per_seq <= 0 || block_size <= 0 || num_heads <= 0 || head_size <= 0) return 0;
+  Kv8Call c{};
+  c.rows = num_rows; c.max_blocks = max_blocks_per_seq;
+  c.cache.heads = num_heads; c.cache.head_size = head_size; c.cache.block_size = block_size;
+  return row_scratch(num_rows, num_heads, head_size, row_splits(c));
+}
+
+extern "C" int aps_kv8_attention(void* out, const void* query, const void* key_cache, const void* value_cache, const float* key_scale,
+                                 const float* value_scale, const int32_t* block_tables, const int32_t* query_start_loc,
+                                 const int32_t* seq_lens, int batch, int64_t num_rows, int max_query_len, int max_blocks_per_seq,
+                                 int num_heads, int head_size, int block_size, int64_t num_blocks, int64_t query_stride,
+                                 int64_t out_stride, int64_t block_stride, int64_t scale_stride, float scale, void* workspace,
+                                 size_t workspace_bytes, int dtype, void* stream) {
+  const Kv8Call c{out, query,
+                  {(const uint8_t*)key_cache, (const uint8_t*)value_cache, key_scale, value_scale, num_blocks, block_stride, scale_stride,
+                   num_heads, head_size, block_size},
+                  block_tables, query_start_loc, seq_lens, batch, max_blocks_per_seq, max_query_len, num_rows, query_stride, out_stride,
+                  scale, dtype};
+  const int st = check_call("kv8_attention", c);
+  if (st != APS_OK || num_rows == 0 || batch == 0) return st;
+  APS_REQUIRE(query_start_loc != nullptr || num_rows == batch, APS_ERR_SHAPE, "kv8_attention: %lld query rows for %d requests",
+              (long long)num_rows, batch);
+  RowArgs a{c, static_cast<int*>(workspace), nullptr, nullptr, row_splits(c), scale * 1.4426950408889634f};
+  const size_t need = row_scratch(num_rows, num_heads, head_size, a.splits);
+  APS_REQUIRE(workspace != nullptr && aligned_to(workspace, 256) && workspace_bytes >= need, APS_ERR_WORKSPACE,
+              "kv8_attention: workspace must be 256-byte aligned and hold %zu bytes (got %zu)", need, workspace_bytes);
+  if (a.splits > 1) {
+    a.ml = reinterpret_cast<float2*>(a.plan + kPlanWords);
+    a.acc = reinterpret_cast<float*>(a.ml + num_rows * num_heads * a.splits);
+  }
+  switch (dtype) {
+    case APS_F32: return rows_by_head<float>(a, (cudaStream_t)stream);
+    case APS_F16: return rows_by_head<__half>(a, (cudaStream_t)stream);
+    default: return rows_by_head<__nv_bfloat16>(a, (cudaStream_t)stream);
+  }
+}

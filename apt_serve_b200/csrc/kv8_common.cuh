@@ -1,0 +1,67 @@
+// The K/V cache in 8 bits: e4m3 numbers with a scale for each block of tokens and head.
+//
+// Row element x of block b and head h is held as the e4m3 number nearest to x / s[b][h] (ties to even); NaN and infinities are held
+// as NaN.  The writer's scales are powers of two, which costs a number with an exponent of its own nothing (its 4 significant bits
+// are the same ones whatever the scale) and makes x / s exact and a block's move to a larger scale a shift of exponents: only what
+// falls below the smallest normal number 2^-6 is rounded again.  Readers take any positive scale.
+#pragma once
+
+#include "attention_common.cuh"
+
+namespace aps {
+
+// A cache and how it is reached.  Strides of the caches in bytes (= elements), of the scales in elements.
+struct Kv8Cache {
+  const uint8_t* key; const uint8_t* value;
+  const float* key_scale; const float* value_scale;
+  int64_t num_blocks, block_stride, scale_stride;
+  int heads, head_size, block_size;
+};
+
+// One attention call.  Row t of the query belongs to the request r with starts[r] <= t < starts[r + 1] (starts == NULL: t itself);
+// the rows of a request are the last of its seq_lens[r] tokens, each attends to the tokens up to itself.
+struct Kv8Call {
+  void* out; const void* query;
+  Kv8Cache cache;
+  const int32_t* tables; const int32_t* starts; const int32_t* seq_lens;
+  int batch, max_blocks, max_rows;   // max_rows: most rows of a request
+  int64_t rows, query_stride, out_stride;
+  float scale;
+  int dtype;
+};
+
+constexpr float kE4m3Max = 448.f;
+
+// The two e4m3 numbers in the low 16 bits as fp16 (exact).
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t codes) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(codes));
+  return r;
+}
+// Four numbers of a word as floats.
+__device__ __forceinline__ void e4m3x4_to_float(uint32_t codes, float* f) {
+  const uint32_t lo = e4m3x2_to_f16x2((uint16_t)codes), hi = e4m3x2_to_f16x2((uint16_t)(codes >> 16));
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
+}
+// To the nearest, ties to even; beyond 448 to 448, NaN to 0x7f.
+__device__ __forceinline__ uint16_t float2_to_e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t float4_to_e4m3x4(const float* f) {
+  return (uint32_t)float2_to_e4m3x2(f[0], f[1]) | (uint32_t)float2_to_e4m3x2(f[2], f[3]) << 16;
+}
+// The smallest power of two s >= 2^-118 with top <= 448 s (448 = 1.75 * 2^8; top finite and not negative).
+__device__ __forceinline__ float e4m3_scale(float top) {
+  const uint32_t u = __float_as_uint(top);
+  const int e = (int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);   // biased; a subnormal top gives the least scale
+  return __uint_as_float((uint32_t)max(e, 127 - 118) << 23);
+}
+
+bool kv8_supported(int dtype, int head_size);
+int check_kv8_cache(const char* op, const Kv8Cache& c, int dtype);
+int read_kv8_status(int* host_status, cudaStream_t stream);   // kv8_write.cu
+
+}  // namespace aps

@@ -119,12 +119,15 @@ class OPTAttention(torch.nn.Module):
     Under tensor parallelism ``hidden_cache`` must be given (a
     ``[2, NB, BS, 1, E]`` tensor replicated per rank); with one rank it defaults
     to ``kv_cache``, the reference's aliasing layout.
+
+    ``cache_config`` (``cache_dtype="fp8"``): the layer's cache is an 8-bit one and ``forward`` is given its scales, ``kv_scale``
+    (fp32 ``[2, NB, H]``, ``CacheEngine.gpu_scale``); batches with hidden-cached requests are then refused.
     """
 
     def __init__(self, embed_dim: int, num_heads: int, qkv_weight: torch.Tensor,
                  qkv_bias: Optional[torch.Tensor], o_weight: torch.Tensor,
                  o_bias: Optional[torch.Tensor], tp_size: int = 1, group=None,
-                 fused=True):
+                 fused=True, cache_config=None):
         super().__init__()
         assert num_heads % tp_size == 0
         self.embed_dim = embed_dim
@@ -133,13 +136,15 @@ class OPTAttention(torch.nn.Module):
         self.scaling = self.head_dim ** -0.5
         self.qkv_proj = QKVParallelLinear(qkv_weight, qkv_bias)
         self.out_proj = RowParallelLinear(o_weight, o_bias, group)
-        self.attn = Attention(self.num_heads, self.head_dim, scale=self.scaling)
+        self.attn = Attention(self.num_heads, self.head_dim, scale=self.scaling, cache_config=cache_config)
         self.fused = fused
 
     def forward(self, hidden_states: torch.Tensor, kv_cache: torch.Tensor,
                 shared_cache: Optional[torch.Tensor], attn_metadata,
-                hidden_cache: Optional[torch.Tensor] = None) -> torch.Tensor:
+                hidden_cache: Optional[torch.Tensor] = None, kv_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
         m = attn_metadata
+        if self.attn.impl.fp8_cache and m.num_hidden_cache_tokens != 0:
+            raise ValueError("hidden-cached requests need a 16-bit or fp32 cache: hidden rows are not held in 8 bits")
         hcache = kv_cache if hidden_cache is None else hidden_cache
         if (self.fused and m.num_hidden_cache_tokens != 0 and m.num_decode_tokens == 0
                 and kv_cache is not None):
@@ -173,7 +178,7 @@ class OPTAttention(torch.nn.Module):
         else:
             qkv, _ = self.qkv_proj(hidden_states)
             q, k, v = qkv.chunk(chunks=3, dim=-1)
-        attn_output = self.attn(q, k, v, kv_cache, shared_cache, m)
+        attn_output = self.attn(q, k, v, kv_cache, shared_cache, m, kv_scale)
         output, _ = self.out_proj(attn_output)
         return output
 

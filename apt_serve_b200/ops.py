@@ -11,17 +11,49 @@ import torch
 from . import _native as N
 
 
+#: what vLLM calls an e4m3 cache
+FP8_CACHE = ("fp8", "fp8_e4m3")
+_FP8_STORAGE = (torch.float8_e4m3fn, torch.uint8)
+
+
+def check_fp8_cache(op: str, key_cache: torch.Tensor, value_cache: torch.Tensor, k_scale, v_scale) -> None:
+    """The two planes ``[NB, BS, H, D]`` of an 8-bit cache (``float8_e4m3fn``, or ``uint8`` holding its bytes) and their scales, fp32
+    ``[NB, H]``, one for each block and head."""
+    if not isinstance(k_scale, torch.Tensor) or not isinstance(v_scale, torch.Tensor):
+        raise ValueError(f"{op}: an 8-bit cache needs k_scale and v_scale tensors")
+    if key_cache.dtype not in _FP8_STORAGE or value_cache.dtype != key_cache.dtype:
+        raise ValueError(f"{op}: an 8-bit cache is float8_e4m3fn or uint8 (got {key_cache.dtype}, {value_cache.dtype})")
+    if key_cache.dim() != 4 or value_cache.shape != key_cache.shape:
+        raise RuntimeError(f"{op}: the caches must be [blocks, block size, heads, head size], alike for keys and values")
+    nb, bs, h, d = key_cache.shape
+    if key_cache.stride()[1:] != (h * d, d, 1) or value_cache.stride() != key_cache.stride():
+        raise RuntimeError(f"{op}: a cache block must be contiguous, and the two caches' strides alike")
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if t.dtype != torch.float32 or t.shape != (nb, h) or t.stride(1) != 1 or t.stride(0) != k_scale.stride(0):
+            raise RuntimeError(f"{op}: {name} must be float32 [{nb}, {h}] with contiguous rows, strides alike")
+
+
 def reshape_and_cache_flash(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
                             value_cache: torch.Tensor, slot_mapping: torch.Tensor,
-                            kv_cache_dtype: str = "auto") -> None:
+                            kv_cache_dtype: str = "auto", k_scale: Optional[torch.Tensor] = None,
+                            v_scale: Optional[torch.Tensor] = None) -> None:
     """``key_cache[slot // BS, slot % BS] = key[t]`` (and value) for ``slot >= 0``.
     ``key`` / ``value``: ``[T, H, D]``; caches ``[NB, BS, H, D]``.  Slots past the last row (a padded mapping) have
-    nothing to store, rows past the last slot nowhere to go."""
-    if kv_cache_dtype != "auto":  # aptserve_flash_attn.py:311-312: no FP8 cache here
+    nothing to store, rows past the last slot nowhere to go.
+
+    ``kv_cache_dtype="fp8"``: the caches hold e4m3 numbers and ``k_scale`` / ``v_scale`` (fp32 ``[NB, H]``) what they are multiplied by, a
+    power of two for each block and head, as small as the finite elements of the rows allow.  The call sets the scales: a block whose first
+    slot is written starts anew, with the scale of the rows it is given (what its other slots hold counts as unwritten); in a block that is
+    written from a later slot on the scale grows if it has to, and the rows it holds already are rounded to it."""
+    if kv_cache_dtype in FP8_CACHE:
+        check_fp8_cache("reshape_and_cache_flash", key_cache, value_cache, k_scale, v_scale)
+    elif kv_cache_dtype != "auto":  # aptserve_flash_attn.py:311-312: no other cache here
         raise ValueError(f"kv_cache_dtype {kv_cache_dtype!r} is not supported")
-    dev = N.require_cuda(key, value, key_cache, value_cache, slot_mapping)
+    dev = N.require_cuda(key, value, key_cache, value_cache, slot_mapping, *((k_scale, v_scale) if kv_cache_dtype != "auto" else ()))
     if slot_mapping.dtype != torch.int64:
         raise RuntimeError("slot_mapping must be int64")
+    if kv_cache_dtype != "auto":
+        return _write_fp8(dev, key, value, key_cache, value_cache, slot_mapping, k_scale, v_scale)
     if key.dtype != key_cache.dtype or value.dtype != value_cache.dtype or key.dtype != value.dtype:
         raise RuntimeError("reshape_and_cache_flash: dtypes differ")
     if key_cache.stride(0) != value_cache.stride(0):
@@ -34,6 +66,26 @@ def reshape_and_cache_flash(key: torch.Tensor, value: torch.Tensor, key_cache: t
             N.ptr(slot_mapping.contiguous()), min(slot_mapping.size(0), key.size(0), value.size(0)), key.size(1), key.size(2),
             key_cache.size(1), key.stride(0), value.stride(0), key_cache.stride(0),
             N.dtype_enum(key), N.current_stream(dev)))
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Elements from row to row of ``[T, H, D]``; of a single row, whose stride can be anything, its width."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def _write_fp8(dev, key, value, key_cache, value_cache, slot_mapping, k_scale, v_scale) -> None:
+    nb, bs, h, d = key_cache.shape
+    if key.dtype != value.dtype:
+        raise RuntimeError("reshape_and_cache_flash: dtypes differ")
+    for t in (key, value):
+        if t.dim() != 3 or t.shape[1:] != (h, d) or t.stride(2) != 1 or (h > 1 and t.stride(1) != d):
+            raise RuntimeError(f"reshape_and_cache_flash: key and value must be [T, {h}, {d}] with contiguous token rows")
+    slots = slot_mapping.contiguous()
+    with N.on_device(dev):
+        N.check(N.lib().aps_kv8_write(
+            key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+            slots.data_ptr(), min(slots.numel(), key.shape[0], value.shape[0]), h, d, bs, nb, _row_stride(key), _row_stride(value),
+            key_cache.stride(0), k_scale.stride(0), N.dtype_enum(key), N.current_stream(dev)))
 
 
 def prefill_cache_write(key: Optional[torch.Tensor], value: Optional[torch.Tensor],

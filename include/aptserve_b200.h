@@ -386,8 +386,8 @@ int aps_reprojection_cycles(const void* workspace, unsigned long long* host_cycl
 
 /*
  * Status of the operations without a workspace on the current device: 0, 1 once a bounded wait on a bulk load of a
- * cache operation ran out (the launch then stopped copying), 2 if aps_derive_private_tables or aps_gather_hidden_rows has met
- * an index outside its tensor since a call that returned 2, or 3 if a bounded wait of aps_prefill_attention has run out
+ * cache operation ran out (the launch then stopped copying), 2 if aps_derive_private_tables, aps_gather_hidden_rows or
+ * aps_kv8_write has met an index outside its tensor since a call that returned 2, or 3 if a bounded wait of aps_prefill_attention has run out
  * (up to 128 rows of a head are then NaN) since the last call that returned 3.  Synchronises `stream`.
  */
 int aps_cache_ops_status(int* host_status, void* stream);
@@ -418,6 +418,46 @@ int aps_selftest_prefill_wait(long long budget_cycles, void* stream);
  * attended rows reads for a tile whose entry in the scratch holds (first, last), with num_pieces pieces in all.
  */
 int aps_selftest_tile_pieces(int first, int last, int num_pieces, int* pieces_out);
+
+/* ------------------------------------------------------------------------ */
+/* The K/V cache in 8 bits (no counterpart in the reference, which refuses   */
+/* any kv_cache_dtype but "auto", fa.py:311-312)                             */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * The caches hold e4m3 numbers, one byte each: [NB, BS, H, D], block_stride bytes from block to block (a multiple of 16),
+ * [BS, H, D] contiguous inside; key_scale / value_scale: fp32 [NB, H], scale_stride elements from block to block.  An element
+ * stands for its number times the scale of its block and head.  block_size: a multiple of 16 up to 1024; head sizes 32, 64, 128, 256.
+ *
+ * aps_kv8_write: rows of K and V ([T, H, D], row strides key_stride / value_stride) into slots as aps_reshape_and_cache has them
+ * (negative: skipped; past the last block: skipped, and the status that aps_cache_ops_status reads is set to 2).  All rows of the
+ * call that go to one block are taken together, in whatever order they come; of two rows for one slot the later one stays.  Needed scale
+ * of a set of rows, for each head: the smallest power of two s >= 2^-118 with |x| <= 448 s for every finite x in them.
+ *  - The block's first slot is among the call's: the block starts anew.  Its scale is the rows' needed one; its other rows keep their
+ *    bytes and count as unwritten.
+ *  - Otherwise the scale becomes the larger of the old one and the needed one; where it grows the block's other rows are rounded to it.
+ * NaN and infinities are stored as NaN and have no part in the scale.
+ */
+int aps_kv8_write(const void* key, const void* value, void* key_cache, void* value_cache, float* key_scale, float* value_scale,
+                  const int64_t* slot_mapping, int64_t num_tokens, int num_heads, int head_size, int block_size,
+                  int64_t num_blocks, int64_t key_stride, int64_t value_stride, int64_t block_stride, int64_t scale_stride,
+                  int dtype, void* stream);
+
+/*
+ * Attention of query rows [num_rows, H, D] over that cache.  Row t belongs to the request r with query_start_loc[r] <= t <
+ * query_start_loc[r + 1] (int32 [batch + 1]; NULL: one row per request, row r is request r's); a request's rows are the last of its
+ * seq_lens[r] tokens, each attends to the tokens up to itself.  A row that attends to none (a length of 0, more rows than tokens) is
+ * zero; rows before the first start and behind the last are left as they are.  max_query_len: no request has more rows.  A table entry
+ * outside [0, num_blocks) is not read: the rows that attend to a token of it become NaN.
+ * workspace: aps_kv8_attention_workspace_bytes(num_rows, ...) bytes, 256-byte aligned; aps_attention_status reads its status word.
+ */
+size_t aps_kv8_attention_workspace_bytes(int64_t num_rows, int max_blocks_per_seq, int block_size, int num_heads, int head_size);
+int aps_kv8_attention(void* out, const void* query, const void* key_cache, const void* value_cache, const float* key_scale,
+                      const float* value_scale, const int32_t* block_tables, const int32_t* query_start_loc,
+                      const int32_t* seq_lens, int batch, int64_t num_rows, int max_query_len, int max_blocks_per_seq,
+                      int num_heads, int head_size, int block_size, int64_t num_blocks, int64_t query_stride,
+                      int64_t out_stride, int64_t block_stride, int64_t scale_stride, float scale, void* workspace,
+                      size_t workspace_bytes, int dtype, void* stream);
 
 /* ------------------------------------------------------------------------ */
 /* Index tensors                                                             */

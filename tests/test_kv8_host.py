@@ -1,0 +1,106 @@
+"""Refusals of the 8-bit cache's entry points, and its cache engine, without a GPU."""
+import ctypes
+
+import pytest
+import torch
+
+from apt_serve_b200 import _native as N
+from apt_serve_b200 import attention as A
+from apt_serve_b200 import ops
+from apt_serve_b200.cache_engine import CacheEngine
+from apt_serve_b200.layers import OPTAttention
+
+E4M3 = torch.float8_e4m3fn
+
+
+def address(offset=0):
+    address.buf = getattr(address, "buf", None) or (ctypes.c_char * 8192)()
+    return (ctypes.addressof(address.buf) + 255) // 256 * 256 + offset
+
+
+def write(**kw):
+    p = address()
+    a = dict(key=p, value=p, kc=p, vc=p, ks=p, vs=p, slots=p, t=2, h=2, d=64, bs=16, nb=4, s_k=128, s_v=128, block=2048, s_s=2, dtype=1)
+    a.update(kw)
+    return N.lib().aps_kv8_write(*a.values(), 0)
+
+
+def attend(**kw):
+    p = address()
+    a = dict(out=p, q=p, kc=p, vc=p, ks=p, vs=p, bt=p, starts=p, sl=p, b=2, t=5, most=3, width=4, h=2, d=64, bs=16, nb=4, s_q=128, s_o=128,
+             block=2048, s_s=2, scale=1.0, ws=p, ws_bytes=1 << 40, dtype=1)
+    a.update(kw)
+    return N.lib().aps_kv8_attention(*a.values(), 0)
+
+
+@pytest.mark.parametrize("status,kw", [
+    (N.APS_ERR_DTYPE, dict(dtype=3)), (N.APS_ERR_UNSUPPORTED, dict(d=96)), (N.APS_ERR_UNSUPPORTED, dict(bs=8)),
+    (N.APS_ERR_UNSUPPORTED, dict(bs=1040, block=1040 * 128)), (N.APS_ERR_SHAPE, dict(h=0)), (N.APS_ERR_SHAPE, dict(t=-1)),
+    (N.APS_ERR_SHAPE, dict(s_k=64)), (N.APS_ERR_SHAPE, dict(block=1024)), (N.APS_ERR_SHAPE, dict(s_s=1)), (N.APS_ERR_SHAPE, dict(nb=1 << 28)),
+    (N.APS_ERR_NULL_POINTER, dict(ks=0)), (N.APS_ERR_NULL_POINTER, dict(slots=0)), (N.APS_ERR_MISALIGNED, dict(kc=address(2))),
+    (N.APS_ERR_MISALIGNED, dict(block=2050)), (N.APS_ERR_MISALIGNED, dict(key=address(1))), (N.APS_OK, dict(t=0, key=0)),
+])
+def test_write_refuses(status, kw):
+    assert write(**kw) == status
+
+
+@pytest.mark.parametrize("status,kw", [
+    (N.APS_ERR_DTYPE, dict(dtype=3)), (N.APS_ERR_UNSUPPORTED, dict(d=80)), (N.APS_ERR_UNSUPPORTED, dict(bs=20, block=4000)),
+    (N.APS_ERR_SHAPE, dict(width=0)), (N.APS_ERR_SHAPE, dict(b=-1)), (N.APS_ERR_SHAPE, dict(s_q=127)), (N.APS_ERR_SHAPE, dict(starts=0)),
+    (N.APS_ERR_SHAPE, dict(width=1 << 28)), (N.APS_ERR_NULL_POINTER, dict(bt=0)), (N.APS_ERR_NULL_POINTER, dict(out=0)),
+    (N.APS_ERR_MISALIGNED, dict(vc=address(8))), (N.APS_ERR_MISALIGNED, dict(block=2056)), (N.APS_ERR_WORKSPACE, dict(width=4000, ws_bytes=64)),
+    (N.APS_ERR_WORKSPACE, dict(width=4000, ws=0)), (N.APS_OK, dict(t=0, q=0)), (N.APS_OK, dict(b=0, bt=0)),
+])
+def test_attention_refuses(status, kw):
+    assert attend(**kw) == status
+
+
+def test_python_refusals():
+    kc, s = torch.zeros(4, 16, 2, 64, dtype=E4M3), torch.zeros(4, 2)
+    x, slots = torch.zeros(3, 2, 64, dtype=torch.float16), torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(ValueError, match="k_scale and v_scale"):
+        ops.reshape_and_cache_flash(x, x, kc, kc, slots, "fp8")
+    with pytest.raises(ValueError, match="float8_e4m3fn or uint8"):
+        ops.reshape_and_cache_flash(x, x, kc.half(), kc.half(), slots, "fp8", s, s)
+    with pytest.raises(ValueError, match="not supported"):
+        ops.reshape_and_cache_flash(x, x, kc, kc, slots, "fp8_e5m2", s, s)
+    for bad in (s[:3], s.double(), torch.zeros(2, 4).t()):
+        with pytest.raises(RuntimeError, match="scale must be float32"):
+            ops.reshape_and_cache_flash(x, x, kc, kc, slots, "fp8", bad, bad)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        ops.reshape_and_cache_flash(x, x, kc[..., :32], kc[..., :32], slots, "fp8", s, s)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        ops.reshape_and_cache_flash(x, x, kc, kc, slots, "fp8", s, s)
+    q, bt, sl = torch.zeros(3, 128), torch.zeros(3, 2, dtype=torch.int32), torch.ones(3, dtype=torch.int32)
+    with pytest.raises(ValueError, match="k_scale and v_scale"):
+        A.paged_decode_attention(q, kc, kc, bt, sl, 1.0)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        A.paged_prefix_attention(q, kc, kc, bt, sl, sl, 1, 1.0, s, s)
+
+
+def test_hidden_cached_requests_are_refused():
+    class Config:
+        cache_dtype, sliding_window = "fp8", None
+    layer = OPTAttention(128, 2, torch.zeros(384, 128), None, torch.zeros(128, 128), None, cache_config=Config)
+
+    class Meta:
+        num_hidden_cache_tokens, num_decode_tokens, num_prefill_tokens = 3, 2, 0
+    with pytest.raises(ValueError, match="hidden-cached"):
+        layer(torch.zeros(2, 128), None, None, Meta)
+    x = torch.zeros(2, 128)
+    with pytest.raises(ValueError, match="hidden-cached"):
+        layer.attn.impl.forward(x, x, x, None, None, Meta)
+
+
+def test_cache_engine_moves_the_scales_with_the_blocks():
+    engine = CacheEngine(2, 4, 64, 16, 8, 4, E4M3, device="cpu", pin_memory=False, hidden_size=512)
+    assert engine.gpu_hidden_cache is None and engine.gpu_cache[0].dtype == E4M3 and engine.gpu_scale[1].shape == (2, 8, 4)
+    engine.gpu_scale[1][:, 3], engine.gpu_cache[1][:, 3] = 2.0, 3.0
+    engine.swap_out(torch.tensor([[3, 1]]))
+    assert (engine.cpu_scale[1][:, 1] == 2).all() and (engine.cpu_cache[1][:, 1].float() == 3).all()
+    engine.swap_in(torch.tensor([[1, 6]]))
+    assert (engine.gpu_scale[1][:, 6] == 2).all() and (engine.gpu_cache[1][:, 6].float() == 3).all()
+    assert CacheEngine.get_cache_block_size(2, 4, 64, 16, E4M3, 512) == 2 * (2 * 16 * 4 * 64 + 2 * 4 * 4)
+    assert CacheEngine.num_blocks_for_budget(10 * 16448, 2, 4, 64, 16, E4M3) == 10
+    with pytest.raises(ValueError, match="shared cache"):
+        CacheEngine(1, 4, 64, 16, 8, 4, E4M3, device="cpu", with_shared_cache=True, pin_memory=False)
