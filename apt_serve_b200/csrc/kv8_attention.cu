@@ -2,6 +2,7 @@
 //
 //   kv8_rows_kernel     CUDA-core arithmetic, one CTA per (query row, head, part of the row's tokens): every query type, head size
 //                       and block stride.  D / 16 lanes cover a row with one 16-byte load each.
+//   (kv8_prefix.cu)     several query rows per request on the tensor cores
 //   kv8_combine_kernel  joins the parts of rows whose tokens were cut.
 // Scores, softmax statistics and sums are fp32; a code times its scale is exact in fp32.
 #include "kv8_common.cuh"
@@ -12,44 +13,16 @@ namespace {
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kRowWarps = 4;
 
-struct RowArgs {
-  Kv8Call c;
-  int* plan;                  // the scratch's header, as the other attention calls have it: its status is set to fine
-  float* acc; float2* ml;     // partials [row][head][split], unless splits == 1
-  int splits;
-  float scale_log2;
-};
-
-// The request of query row t, and how many tokens the row attends to (none: a zero row).  False: the row belongs to no request.
-__device__ __forceinline__ bool find_row(const Kv8Call& c, int64_t t, int& req, int& keys) {
-  if (c.starts == nullptr) {
-    req = (int)t;
-    keys = max(0, min(c.seq_lens[req], c.max_blocks * c.cache.block_size));
-    return true;
-  }
-  if (t < c.starts[0] || t >= c.starts[c.batch]) return false;
-  int lo = 0, hi = c.batch;   // starts[lo] <= t < starts[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (c.starts[mid] <= t) lo = mid; else hi = mid;
-  }
-  req = lo;
-  const int ctx = max(0, min(c.seq_lens[req], c.max_blocks * c.cache.block_size));
-  keys = max(0, ctx - c.starts[req + 1] + (int)t + 1);
-  return true;
-}
-
 template <typename T, int D>
 __global__ void __launch_bounds__(kRowWarps * 32)
-kv8_rows_kernel(const RowArgs a) {
+kv8_rows_kernel(const Kv8Call c, const Kv8Parts a) {
   constexpr int kLanes = D / 16, kTok = 32 / kLanes, kLoads = 4;   // lanes per row, rows per load, loads at a time
-  const Kv8Call& c = a.c;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % kLanes, tsel = lane / kLanes;
   const int64_t t = blockIdx.x / a.splits;
   const int split = (int)(blockIdx.x % a.splits), h = blockIdx.y;
   if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) a.plan[kPlanStatus] = kStatusOk;
   int req, keys;
-  if (!find_row(c, t, req, keys)) return;
+  if (!kv8_find_row(c, t, req, keys)) return;
   const int per = ((keys + a.splits - 1) / a.splits + 15) / 16 * 16;
   const int begin = min(keys, split * per), end = min(keys, begin + per);
   const int32_t* table = c.tables + (int64_t)req * c.max_blocks;
@@ -152,14 +125,13 @@ kv8_rows_kernel(const RowArgs a) {
 // One warp per (query row, head).
 template <typename T>
 __global__ void __launch_bounds__(256)
-kv8_combine_kernel(const RowArgs a) {
-  const Kv8Call& c = a.c;
+kv8_combine_kernel(const Kv8Call c, const Kv8Parts a) {
   const int lane = threadIdx.x & 31, d = c.cache.head_size;
   const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (unit >= c.rows * c.cache.heads) return;
   const int64_t t = unit / c.cache.heads, h = unit % c.cache.heads;
   int req, keys;
-  if (!find_row(c, t, req, keys)) return;
+  if (!kv8_find_row(c, t, req, keys)) return;
   const float2* ml = a.ml + unit * a.splits;
   const float* acc = a.acc + unit * a.splits * d;
   float top = -INFINITY, sum = 0.f;
@@ -173,7 +145,8 @@ kv8_combine_kernel(const RowArgs a) {
   T* out = static_cast<T*>(c.out) + t * c.out_stride + h * d;
   for (int e = lane; e < d; e += 32) {
     float x = 0.f;
-    for (int i = 0; i < a.splits; ++i) x = fmaf(exp2f(ml[i].x - ref), acc[(int64_t)i * d + e], x);
+    for (int i = 0; i < a.splits; ++i)
+      if (ml[i].x != -INFINITY) x = fmaf(exp2f(ml[i].x - ref), acc[(int64_t)i * d + e], x);   // a part without tokens has no acc
     out[e] = Elem<T>::from_float(keys == 0 ? 0.f : x / sum);
   }
 }
@@ -186,29 +159,44 @@ int row_splits(const Kv8Call& c) {
   return (int)(n < 1 ? 1 : n > 1024 ? 1024 : n);
 }
 
-size_t row_scratch(int64_t rows, int heads, int head_size, int splits) {
-  return kPlanWords * sizeof(int) + (splits == 1 ? 0 : (size_t)rows * heads * splits * (head_size + 2) * sizeof(float));
+// The scratch: header, maxima and sums, weighted values (16-byte stores).
+size_t part_acc_at(int64_t rows, int heads, int splits) {
+  return align_up(kPlanWords * sizeof(int) + (size_t)rows * heads * splits * sizeof(float2), 256);
 }
-
-template <typename T, int D>
-int launch_rows(const RowArgs& a, cudaStream_t stream) {
-  const int64_t grid = a.c.rows * a.splits;
-  APS_REQUIRE(grid < (int64_t(1) << 31), APS_ERR_SHAPE, "kv8_attention: too many rows");
-  kv8_rows_kernel<T, D><<<dim3((unsigned)grid, a.c.cache.heads), kRowWarps * 32, 0, stream>>>(a);
-  int st = launch_status("kv8_rows_kernel");
-  if (st != APS_OK || a.splits == 1) return st;
-  kv8_combine_kernel<T><<<(unsigned)((a.c.rows * a.c.cache.heads + 7) / 8), 256, 0, stream>>>(a);
-  return launch_status("kv8_combine_kernel");
+size_t part_scratch(int64_t rows, int heads, int head_size, int splits) {
+  if (splits == 1) return kPlanWords * sizeof(int);
+  return part_acc_at(rows, heads, splits) + (size_t)rows * heads * splits * head_size * sizeof(float);
 }
 
 template <typename T>
-int rows_by_head(const RowArgs& a, cudaStream_t stream) {
-  switch (a.c.cache.head_size) {
-    case 32: return launch_rows<T, 32>(a, stream);
-    case 64: return launch_rows<T, 64>(a, stream);
-    case 128: return launch_rows<T, 128>(a, stream);
-    default: return launch_rows<T, 256>(a, stream);
+int launch_parts_combine(const Kv8Call& c, const Kv8Parts& a, cudaStream_t stream) {
+  if (a.splits == 1) return APS_OK;
+  kv8_combine_kernel<T><<<(unsigned)((c.rows * c.cache.heads + 7) / 8), 256, 0, stream>>>(c, a);
+  return launch_status("kv8_combine_kernel");
+}
+
+template <typename T, int D>
+int launch_rows(const Kv8Call& c, const Kv8Parts& a, cudaStream_t stream) {
+  const int64_t grid = c.rows * a.splits;
+  APS_REQUIRE(grid < (int64_t(1) << 31), APS_ERR_SHAPE, "kv8_attention: too many rows");
+  kv8_rows_kernel<T, D><<<dim3((unsigned)grid, c.cache.heads), kRowWarps * 32, 0, stream>>>(c, a);
+  return launch_status("kv8_rows_kernel");
+}
+
+template <typename T>
+int attend(const Kv8Call& c, const Kv8Parts& a, bool tiles, cudaStream_t stream) {
+  int st;
+  if (tiles) {
+    st = launch_kv8_tiles(c, a, stream);
+  } else {
+    switch (c.cache.head_size) {
+      case 32: st = launch_rows<T, 32>(c, a, stream); break;
+      case 64: st = launch_rows<T, 64>(c, a, stream); break;
+      case 128: st = launch_rows<T, 128>(c, a, stream); break;
+      default: st = launch_rows<T, 256>(c, a, stream); break;
+    }
   }
+  return st != APS_OK ? st : launch_parts_combine<T>(c, a, stream);
 }
 
 int check_call(const char* op, const Kv8Call& c) {
@@ -240,7 +228,8 @@ extern "C" size_t aps_kv8_attention_workspace_bytes(int64_t num_rows, int max_bl
   Kv8Call c{};
   c.rows = num_rows; c.max_blocks = max_blocks_per_seq;
   c.cache.heads = num_heads; c.cache.head_size = head_size; c.cache.block_size = block_size;
-  return row_scratch(num_rows, num_heads, head_size, row_splits(c));
+  const int by_rows = row_splits(c), by_tiles = kv8_tile_splits(c);
+  return part_scratch(num_rows, num_heads, head_size, by_rows > by_tiles ? by_rows : by_tiles);
 }
 
 extern "C" int aps_kv8_attention(void* out, const void* query, const void* key_cache, const void* value_cache, const float* key_scale,
@@ -258,17 +247,18 @@ extern "C" int aps_kv8_attention(void* out, const void* query, const void* key_c
   if (st != APS_OK || num_rows == 0 || batch == 0) return st;
   APS_REQUIRE(query_start_loc != nullptr || num_rows == batch, APS_ERR_SHAPE, "kv8_attention: %lld query rows for %d requests",
               (long long)num_rows, batch);
-  RowArgs a{c, static_cast<int*>(workspace), nullptr, nullptr, row_splits(c), scale * 1.4426950408889634f};
-  const size_t need = row_scratch(num_rows, num_heads, head_size, a.splits);
+  const bool tiles = kv8_tiles_take(c);
+  Kv8Parts a{static_cast<int*>(workspace), nullptr, nullptr, tiles ? kv8_tile_splits(c) : row_splits(c), scale * 1.4426950408889634f};
+  const size_t need = part_scratch(num_rows, num_heads, head_size, a.splits);
   APS_REQUIRE(workspace != nullptr && aligned_to(workspace, 256) && workspace_bytes >= need, APS_ERR_WORKSPACE,
               "kv8_attention: workspace must be 256-byte aligned and hold %zu bytes (got %zu)", need, workspace_bytes);
   if (a.splits > 1) {
     a.ml = reinterpret_cast<float2*>(a.plan + kPlanWords);
-    a.acc = reinterpret_cast<float*>(a.ml + num_rows * num_heads * a.splits);
+    a.acc = reinterpret_cast<float*>(static_cast<char*>(workspace) + part_acc_at(num_rows, num_heads, a.splits));
   }
   switch (dtype) {
-    case APS_F32: return rows_by_head<float>(a, (cudaStream_t)stream);
-    case APS_F16: return rows_by_head<__half>(a, (cudaStream_t)stream);
-    default: return rows_by_head<__nv_bfloat16>(a, (cudaStream_t)stream);
+    case APS_F32: return attend<float>(c, a, tiles, (cudaStream_t)stream);
+    case APS_F16: return attend<__half>(c, a, tiles, (cudaStream_t)stream);
+    default: return attend<__nv_bfloat16>(c, a, tiles, (cudaStream_t)stream);
   }
 }

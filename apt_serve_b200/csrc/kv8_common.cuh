@@ -60,6 +60,39 @@ __device__ __forceinline__ float e4m3_scale(float top) {
   return __uint_as_float((uint32_t)max(e, 127 - 118) << 23);
 }
 
+// Where the parts of rows whose tokens are cut go: [row][head][split], and the header of the scratch (PlanWord).
+struct Kv8Parts {
+  int* plan;
+  float2* ml;                // maximum of the scores (log2) and sum of the weights relative to it; nothing attended: (-infinity, 0)
+  float* acc;                // weighted values, relative to that maximum
+  int splits;                // 1: the output is written directly
+  float scale_log2;
+};
+
+// The request of query row t, and how many tokens the row attends to (none: a zero row).  False: the row belongs to no request.
+__device__ __forceinline__ bool kv8_find_row(const Kv8Call& c, int64_t t, int& req, int& keys) {
+  if (c.starts == nullptr) {
+    req = (int)t;
+    keys = max(0, min(c.seq_lens[req], c.max_blocks * c.cache.block_size));
+    return true;
+  }
+  if (t < c.starts[0] || t >= c.starts[c.batch]) return false;
+  int lo = 0, hi = c.batch;   // starts[lo] <= t < starts[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (c.starts[mid] <= t) lo = mid; else hi = mid;
+  }
+  req = lo;
+  const int ctx = max(0, min(c.seq_lens[req], c.max_blocks * c.cache.block_size));
+  keys = max(0, ctx - c.starts[req + 1] + (int)t + 1);
+  return true;
+}
+
+// Query rows by tiles of 128 on the tensor cores (kv8_prefix.cu).
+bool kv8_tiles_take(const Kv8Call& c);
+int kv8_tile_splits(const Kv8Call& c);
+int launch_kv8_tiles(const Kv8Call& c, const Kv8Parts& parts, cudaStream_t stream);
+
 bool kv8_supported(int dtype, int head_size);
 int check_kv8_cache(const char* op, const Kv8Cache& c, int dtype);
 int read_kv8_status(int* host_status, cudaStream_t stream);   // kv8_write.cu

@@ -1,0 +1,424 @@
+// Several query rows per request over the 8-bit cache (kv8_common.cuh), fp16 / bf16 queries, head sizes 64 and 128.
+//
+// One CTA per (128 query rows of a request, head, part of the tokens), two CTAs per SM, key tiles of 64 tokens up to the diagonal:
+//   four warps turn the tile's codes into fp16 on their way from the cache to shared memory (every e4m3 number is an fp16 number)
+//   S = Q K^T   tcgen05, M = 128 rows, N = 64 tokens, both operands K-major in shared memory, S in one of two buffers of tensor memory
+//   a thread per query row turns its row of S into weights, in fp16 over S
+//   O += P V    tcgen05, A = P from tensor memory, B = V MN-major
+// The scales never meet a rounded number: a block's key scale multiplies the row's fp32 scores, its value scale the fp32 weight before
+// that is rounded to fp16 (11 bits; the cache itself holds 4).  The two have running references of their own: m, the maximum of the
+// scores (log2), for the sum of the weights l, and R, the maximum of score + log2(value scale), for the weights that meet V: so a block
+// of small values that has all the weight fills fp16's range like any other.  O stays in tensor memory and is rescaled only when R has
+// grown by more than 2^8.  The output is O 2^(R - m) / l.
+// bf16 queries become fp16 with a power of two for each row, which leaves 2^-40 of the row's largest element.
+#include "kv8_common.cuh"
+#include "sm100.cuh"
+
+#include <type_traits>
+
+namespace aps {
+namespace {
+
+constexpr int kRows = 128, kKeys = 64, kGroups = kKeys / 16, kSoftWarp = 1, kCopyWarp = 5, kThreads = 9 * 32;
+constexpr float kSlack = 8.f;   // log2 of how much R may have grown before O is rescaled
+constexpr float kUp = 7.f;      // log2 of what the weights are kept at: 2^15 at most
+constexpr int kStatusTileWait = 6;
+
+struct Aux {
+  uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2];   // tile j: entry j & 1, phase j >> 1
+  float4 scales[4][kGroups];      // tile j & 3: key scale, log2 of the value scale
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+__device__ __forceinline__ void mma_tmem_a(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+      "mov.b64 db, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void st_shared16(uint32_t addr, const uint32_t* w) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+}
+
+template <int D> constexpr size_t tile_smem() { return 1024 + (size_t)(kRows + 4 * kKeys) * D * 2; }
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 2)
+kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, int vec) {
+  constexpr uint32_t kQSlab = kRows * 128, kSlab = kKeys * 128, kQBytes = D / 64 * kQSlab, kTileBytes = D / 64 * kSlab;
+  constexpr uint32_t kCols = 256, kO = 128;            // tensor memory: two buffers of S (and P over it), then O
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t q_at = (smem_u32(smem_raw) + 1023) & ~1023u, k_at = q_at + kQBytes, v_at = k_at + 2 * kTileBytes;
+  __shared__ Aux aux;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const int head = blockIdx.y, req = blockIdx.z, splits = parts.splits, split = blockIdx.x % splits;
+  if (blockIdx.x == 0 && head == 0 && req == 0 && threadIdx.x == 0) parts.plan[kPlanStatus] = kStatusOk;
+  const int start = c.starts[req], n_rows = c.starts[req + 1] - start;
+  const int row0 = (int)(gridDim.x / splits - 1 - blockIdx.x / splits) * kRows;    // the rows with the most tokens first
+  if (row0 >= n_rows) return;
+  const int bs = c.cache.block_size, ctx = max(0, min(c.seq_lens[req], c.max_blocks * bs));
+  const int first = ctx - n_rows + row0;                                 // own position of the CTA's first row
+  const int end = first + min(kRows, n_rows - row0);                     // tokens that its last row attends to, if any
+  const int all_tiles = max(0, (end + kKeys - 1) / kKeys), per = (all_tiles + splits - 1) / splits;
+  const int tile0 = min(all_tiles, split * per), n_tiles = min(all_tiles, tile0 + per) - tile0;
+  const int key0 = tile0 * kKeys;
+  if (threadIdx.x == 0) {
+    mbar_init(&aux.q_full, 4);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&aux.k_full[i], 4); mbar_init(&aux.v_full[i], 4); mbar_init(&aux.k_empty[i], 1); mbar_init(&aux.v_empty[i], 1);
+      mbar_init(&aux.s_full[i], 1); mbar_init(&aux.p_full[i], 4);
+    }
+    aux.abort_flag = 0;
+    mbar_init_fence();
+  }
+  if (warp == 0) tmem_alloc(&aux.tmem_base, kCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = aux.tmem_base;
+  volatile int* abort_flag = &aux.abort_flag;
+  int* status = parts.plan + kPlanStatus;
+  auto wait = [&](uint64_t* bars, int tile) {
+    return mbar_wait_warp(smem_u32(&bars[tile & 1]), (uint32_t)(tile >> 1) & 1u, abort_flag, status, kStatusTileWait, lane);
+  };
+  auto arrive = [&](uint64_t* bar) {   // what the warp has written to shared memory is the tensor cores'
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) mbar_arrive_addr(smem_u32(bar));
+  };
+  bool ok = true;
+  if (warp >= kCopyWarp) {
+    // ---- codes to fp16 ----
+    constexpr int kPieces = D / 16, kAtOnce = 128 / kPieces, kLoads = kKeys / kAtOnce;   // 16-byte pieces of a row, rows at once
+    const int at = threadIdx.x - kCopyWarp * 32, piece = at % kPieces, r0 = at / kPieces;
+    const int32_t* table = c.tables + (int64_t)req * c.max_blocks;
+    const int64_t row_bytes = (int64_t)c.cache.heads * D, column = (int64_t)head * D + piece * 16;
+    auto store = [&](uint32_t tile, int row, const uint4& codes) {
+      uint32_t h[8];
+      const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        h[2 * i] = e4m3x2_to_f16x2((uint16_t)w[i]);
+        h[2 * i + 1] = e4m3x2_to_f16x2((uint16_t)(w[i] >> 16));
+      }
+      const uint32_t base = tile + piece / 4 * kSlab + row * 128;
+      const int odd = piece / 4 & 1;   // the second slab's pieces in the other order: 8 lanes, 8 different bank groups
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int half = i ^ odd;
+        uint32_t v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = half ? h[4 + e] : h[e];
+        st_shared16(base + (((piece % 4 * 2 + half) ^ (row & 7)) << 4), v);
+      }
+    };
+    for (int j = 0; j < n_tiles; ++j) {
+      uint4 k[kLoads], v[kLoads];
+      float4 s = make_float4(0.f, -INFINITY, 0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int tok = key0 + j * kKeys + r0 + i * kAtOnce;
+        k[i] = v[i] = make_uint4(0, 0, 0, 0);
+        if (tok < end) {
+          const int64_t block = table[tok / bs];
+          if (block >= 0 && block < c.cache.num_blocks) {
+            const int64_t from = block * c.cache.block_stride + tok % bs * row_bytes + column;
+            k[i] = *reinterpret_cast<const uint4*>(c.cache.key + from);
+            v[i] = *reinterpret_cast<const uint4*>(c.cache.value + from);
+          }
+        }
+      }
+      if (at < kGroups) {
+        const int tok = key0 + j * kKeys + at * 16;
+        if (tok < end) {
+          const int64_t block = table[tok / bs];
+          s.x = __int_as_float(0x7fc00000);   // a block outside the cache: the scores of its tokens are NaN
+          if (block >= 0 && block < c.cache.num_blocks) {
+            s.x = c.cache.key_scale[block * c.cache.scale_stride + head];
+            s.y = log2f(c.cache.value_scale[block * c.cache.scale_stride + head]);
+          }
+        }
+      }
+      const int i2 = j & 1;
+      if (j > 1 && !wait(aux.k_empty, j - 2)) { ok = false; break; }
+      if (at < kGroups) aux.scales[j & 3][at] = s;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) store(k_at + i2 * kTileBytes, r0 + i * kAtOnce, k[i]);
+      arrive(&aux.k_full[i2]);
+      if (j > 1 && !wait(aux.v_empty, j - 2)) { ok = false; break; }
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) store(v_at + i2 * kTileBytes, r0 + i * kAtOnce, v[i]);
+      arrive(&aux.v_full[i2]);
+    }
+  } else if (warp == 0) {
+    // ---- products ----
+    constexpr uint32_t s_idesc = mma_idesc(0, 128, kKeys, false);
+    constexpr uint32_t o_idesc = mma_idesc(0, 128, D, false) | (1u << 16);   // B is MN-major
+    auto scores = [&](int j) {   // S of tile j
+      const int i = j & 1;
+      // the buffer still holds the weights of tile j - 2
+      if (!wait(aux.k_full, j) || (j > 1 && !wait(aux.v_empty, j - 2))) return false;
+      tc_fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          tc_mma_cta(tmem + i * kKeys, desc_lo(q_at + k / 4 * kQSlab + k % 4 * 32, 16), desc_hi(1024, true),
+                     desc_lo(k_at + i * kTileBytes + k / 4 * kSlab + k % 4 * 32, 16), desc_hi(1024, true), s_idesc, k != 0);
+        tc_commit_cta(smem_u32(&aux.k_empty[i]));
+        tc_commit_cta(smem_u32(&aux.s_full[i]));
+      }
+      __syncwarp();
+      return true;
+    };
+    if (n_tiles > 0)
+      ok = mbar_wait_warp(smem_u32(&aux.q_full), 0, abort_flag, status, kStatusTileWait, lane) && scores(0);
+    for (int j = 0; j < n_tiles && ok; ++j) {
+      const int i = j & 1;
+      if ((j + 1 < n_tiles && !scores(j + 1)) || !wait(aux.v_full, j) || !wait(aux.p_full, j)) { ok = false; break; }
+      tc_fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < kKeys / 16; ++k)
+          mma_tmem_a(tmem + kO, tmem + i * kKeys + k * 8, desc_lo(v_at + i * kTileBytes + k * 2048, kSlab), desc_hi(1024, true), o_idesc,
+                     j > 0 || k != 0);
+        tc_commit_cta(smem_u32(&aux.v_empty[i]));
+      }
+      __syncwarp();
+    }
+  } else {
+    // ---- softmax: a thread per row; the warp's quarter of tensor memory is its number modulo 4 ----
+    const int quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16), o_at = lanes + kO;
+    const int64_t t = (int64_t)start + row0 + row;
+    const bool mine = row0 + row < n_rows && t >= 0 && t < c.rows;
+    float up = 1.f;   // what the row's scores are multiplied by for its query's fp16 form
+    {
+      const T* src = static_cast<const T*>(c.query) + (mine ? t : 0) * c.query_stride + (int64_t)head * D;
+      auto eight = [&](int e, float* x) {
+        if (!mine) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = 0.f;
+        } else if (vec) {
+          Vec16<T>::unpack(*reinterpret_cast<const uint4*>(src + e), x);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = Elem<T>::to_float(src[e + i]);
+        }
+      };
+      float down = 1.f;
+      if (std::is_same<T, __nv_bfloat16>::value) {
+        float top = 0.f;
+#pragma unroll 2
+        for (int e = 0; e < D; e += 8) {
+          float x[8];
+          eight(e, x);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (fabsf(x[i]) <= 3.402823466e38f) top = fmaxf(top, fabsf(x[i]));
+        }
+        // the largest element to 2^14 ... 2^15; factors within fp32's normal range
+        const int p = min(120, 127 + 14 - (int)(__float_as_uint(top) >> 23));
+        down = __uint_as_float((uint32_t)(127 + p) << 23);
+        up = __uint_as_float((uint32_t)(127 - p) << 23);
+      }
+#pragma unroll 2
+      for (int e = 0; e < D; e += 8) {
+        float x[8];
+        eight(e, x);
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = half2_bits(x[2 * i] * down, x[2 * i + 1] * down);
+        st_shared16(q_at + e / 64 * kQSlab + row * 128 + (((e / 8 & 7) ^ (row & 7)) << 4), w);
+      }
+      arrive(&aux.q_full);
+    }
+    const float coef = parts.scale_log2 * up;
+    float m = -INFINITY, l = 0.f, ref = -INFINITY;
+    for (int j = 0; j < n_tiles; ++j) {
+      const uint32_t s_at = lanes + (j & 1) * kKeys;
+      const int seen = first + row - key0 - j * kKeys;   // the last token of the tile that the row attends to
+      const bool diagonal = key0 + j * kKeys + kKeys - 1 > first;
+      if (!wait(aux.s_full, j) || !wait(aux.v_full, j)) { ok = false; break; }   // the scales are written before V
+      tc_fence_after();
+      uint32_t v[kKeys];
+      tmem_ld32(s_at, v);
+      tmem_ld32(s_at + 32, v + 32);
+      tmem_ld_wait();
+      if (diagonal) {
+#pragma unroll
+        for (int i = 0; i < kKeys; ++i)
+          if (i > seen) v[i] = 0xff800000u;   // -infinity
+      }
+      float by[kGroups], lv[kGroups], m_new = m, r_new = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < kGroups; ++b) {
+        const float4 s = aux.scales[j & 3][b];
+        by[b] = coef * s.x;
+        lv[b] = s.y;
+        float tops[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) tops[i & 1] = fmaxf(tops[i & 1], __uint_as_float(v[16 * b + i]));
+        const float top = fmaxf(tops[0], tops[1]) * by[b];   // NaN (-infinity times a scale of 0) counts as none
+        m_new = fmaxf(m_new, top);
+        r_new = fmaxf(r_new, top + lv[b]);
+      }
+      if (j == 0) {
+        ref = r_new;
+      } else {
+        const bool move = r_new > ref && !(r_new - ref <= kSlack);
+        if (__any_sync(0xffffffffu, move)) {
+          if (!wait(aux.v_empty, j - 1)) { ok = false; break; }   // O is as the last tile left it
+          tc_fence_after();
+          const float down = move && ref != -INFINITY ? ex2(ref - r_new) : 1.f;
+          if (move) ref = r_new;
+#pragma unroll
+          for (int d = 0; d < D; d += 16) {
+            uint32_t o[16];
+            tmem_ld16(o_at + d, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * down);
+            tmem_st16(o_at + d, o);
+          }
+        }
+      }
+      const float shift = m_new == -INFINITY ? 0.f : m_new, base = shift - (ref == -INFINITY ? 0.f : ref) + kUp;
+      l *= m == -INFINITY ? 0.f : ex2(m - shift);
+      m = m_new;
+      float sums[2] = {0.f, 0.f};
+#pragma unroll
+      for (int b = 0; b < kGroups; ++b) {
+        const float gain = ex2(fminf(base + lv[b], 126.f));
+#pragma unroll
+        for (int i = 16 * b; i < 16 * b + 16; i += 2) {
+          float x = fmaf(__uint_as_float(v[i]), by[b], -shift), y = fmaf(__uint_as_float(v[i + 1]), by[b], -shift);
+          if (diagonal) {   // -infinity times a scale that is 0 or NaN is not
+            x = i > seen ? -INFINITY : x;
+            y = i + 1 > seen ? -INFINITY : y;
+          }
+          x = ex2(x);
+          y = ex2(y);
+          sums[0] += x;
+          sums[1] += y;
+          v[i / 2] = half2_bits(x * gain, y * gain);
+        }
+      }
+      l += sums[0] + sums[1];
+      tmem_st16(s_at, v);
+      tmem_st16(s_at + 16, v + 16);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_addr(smem_u32(&aux.p_full[j & 1]));
+    }
+    ok = ok && (n_tiles == 0 || wait(aux.v_empty, n_tiles - 1));
+    tc_fence_after();
+    const float bad = __int_as_float(0x7fc00000);
+    // O is relative to 2^(ref - kUp), the sum and the parts to 2^m
+    float by = ref == -INFINITY ? 0.f : ex2(ref - kUp - (m == -INFINITY ? 0.f : m));
+    const bool none = first + row < 0;    // a row before the first token
+    const int64_t unit = (t * c.cache.heads + head) * splits + split;
+    if (splits == 1) by /= l;             // nothing but scores of -infinity: NaN
+    if (!ok) by = bad;
+    if (none) by = 0.f;
+    T* out = static_cast<T*>(c.out) + t * c.out_stride + (int64_t)head * D;
+#pragma unroll
+    for (int d = 0; d < D; d += 16) {
+      uint32_t o[16];
+      if (n_tiles > 0) {
+        tmem_ld16(o_at + d, o);
+        tmem_ld_wait();
+      }
+      float x[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = none || n_tiles == 0 ? 0.f : __uint_as_float(o[i]) * by;
+      if (mine && splits > 1) {
+        float* dst = parts.acc + unit * D + d;
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+      } else if (mine && vec) {
+        struct alignas(16) Eight { T x[8]; };
+#pragma unroll
+        for (int i = 0; i < 16; i += 8) {
+          Eight e;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) e.x[k] = Elem<T>::from_float(x[i + k]);
+          *reinterpret_cast<Eight*>(out + d + i) = e;
+        }
+      } else if (mine) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) out[d + i] = Elem<T>::from_float(x[i]);
+      }
+    }
+    if (splits > 1 && mine) parts.ml[unit] = make_float2(ok ? m : 0.f, ok ? l : bad);
+  }
+  if (!ok) {   // products still in flight get a bounded time to end
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000LL) { }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) { tc_fence_after(); tmem_free(tmem, kCols); }
+}
+
+template <typename T, int D>
+int launch(const Kv8Call& c, const Kv8Parts& parts, cudaStream_t stream) {
+  static bool done[64] = {false};
+  auto kernel = kv8_tile_kernel<T, D>;
+  int dev = 0;
+  APS_CUDA(cudaGetDevice(&dev));
+  APS_REQUIRE(dev >= 0 && dev < 64, APS_ERR_CUDA, "device index %d out of range", dev);
+  if (!done[dev]) {
+    APS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tile_smem<D>()));
+    APS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+    done[dev] = true;
+  }
+  const int vec = aligned_to(c.query, 16) && aligned_to(c.out, 16) && c.query_stride % 8 == 0 && c.out_stride % 8 == 0;
+  const int blocks = (c.max_rows + kRows - 1) / kRows;
+  kernel<<<dim3(blocks * parts.splits, c.cache.heads, c.batch), kThreads, tile_smem<D>(), stream>>>(c, parts, vec);
+  return launch_status("kv8_tile_kernel");
+}
+
+}  // namespace
+
+bool kv8_tiles_take(const Kv8Call& c) {
+  // the maximum is taken of the raw scores: a scale that is not positive would need their minimum
+  return c.starts != nullptr && c.max_rows > 1 && (c.dtype == APS_F16 || c.dtype == APS_BF16) &&
+         (c.cache.head_size == 64 || c.cache.head_size == 128) && c.scale >= 1.17549435e-38f && c.scale < 1.70141183e38f && c.batch <= 65535;
+}
+
+// Parts that the tokens of a tile of rows are cut into: enough CTAs for two per SM, four key tiles each at least.
+int kv8_tile_splits(const Kv8Call& c) {
+  const int64_t tiles = ((int64_t)c.max_blocks * c.cache.block_size + kKeys - 1) / kKeys;
+  const int64_t units = (c.rows + kRows - 1) / kRows * c.cache.heads;   // at least
+  int64_t n = ((int64_t)sm_count() * 2 + units - 1) / units;
+  if (n > (tiles + 3) / 4) n = (tiles + 3) / 4;
+  return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+}
+
+int launch_kv8_tiles(const Kv8Call& c, const Kv8Parts& parts, cudaStream_t stream) {
+  if (c.dtype == APS_BF16)
+    return c.cache.head_size == 128 ? launch<__nv_bfloat16, 128>(c, parts, stream) : launch<__nv_bfloat16, 64>(c, parts, stream);
+  return c.cache.head_size == 128 ? launch<__half, 128>(c, parts, stream) : launch<__half, 64>(c, parts, stream);
+}
+
+}  // namespace aps
