@@ -203,8 +203,8 @@ int check_call(const char* op, const Kv8Call& c) {
   const int st = check_kv8_cache(op, c.cache, c.dtype);
   if (st != APS_OK) return st;
   APS_REQUIRE(c.batch >= 0 && c.rows >= 0 && c.max_blocks > 0 && c.max_rows >= 0, APS_ERR_SHAPE, "%s: bad sizes", op);
-  APS_REQUIRE((int64_t)c.max_blocks * c.cache.block_size < (int64_t(1) << 31) && c.rows < (int64_t(1) << 31), APS_ERR_SHAPE,
-              "%s: more than 2^31 tokens", op);
+  APS_REQUIRE((int64_t)c.max_blocks * c.cache.block_size < (int64_t(1) << 30) && c.rows < (int64_t(1) << 31), APS_ERR_SHAPE,
+              "%s: tables for more than 2^30 tokens", op);
   if (c.rows == 0 || c.batch == 0) return APS_OK;
   APS_REQUIRE(c.out && c.query && c.tables && c.seq_lens && c.cache.key && c.cache.value && c.cache.key_scale && c.cache.value_scale,
               APS_ERR_NULL_POINTER, "%s: null pointer", op);

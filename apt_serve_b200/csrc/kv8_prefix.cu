@@ -19,14 +19,18 @@
 namespace aps {
 namespace {
 
-constexpr int kRows = 128, kKeys = 64, kGroups = kKeys / 16, kSoftWarp = 1, kCopyWarp = 5, kThreads = 9 * 32;
+constexpr int kRows = 128, kKeys = 64, kGroups = kKeys / 16, kCopyWarps = 4, kSoftWarp = 1 + kCopyWarps;
 constexpr float kSlack = 8.f;   // log2 of how much R may have grown before O is rescaled
 constexpr float kUp = 7.f;      // log2 of what the weights are kept at: 2^15 at most
 constexpr int kStatusTileWait = 6;
 
+// kTiles: tiles of 128 rows that share the CTA's keys and values.
+template <int kTiles>
 struct Aux {
-  uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2];   // tile j: entry j & 1, phase j >> 1
-  float4 scales[4][kGroups];      // tile j & 3: key scale, log2 of the value scale
+  // key tile j: entry j & 1, phase j >> 1
+  uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[kTiles][2], p_full[kTiles][2], o_done[kTiles][2];
+  uint64_t scales_full[4];        // entry j & 3, phase j >> 2: written again only after the weights of tile j + 1
+  float2 scales[4][kGroups];      // key scale, log2 of the value scale
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -51,6 +55,35 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Not moved behind the waits that follow it.
+__device__ __forceinline__ uint4 ld_ahead(const uint8_t* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+// Two at a time.
+__device__ __forceinline__ float2 fma2(float2 a, float b, float c) {
+  uint64_t x, y, z;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(y) : "f"(b));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(z) : "f"(c));
+  asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(x) : "l"(y), "l"(z));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(x));
+  return a;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t x, y;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(b.x), "f"(b.y));
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(y));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(x));
+  return a;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
 __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -59,34 +92,40 @@ __device__ __forceinline__ void st_shared16(uint32_t addr, const uint32_t* w) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
 }
 
-template <int D> constexpr size_t tile_smem() { return 1024 + (size_t)(kRows + 4 * kKeys) * D * 2; }
+template <int D, int kTiles> constexpr size_t tile_smem() { return 1024 + (size_t)(kTiles * kRows + 4 * kKeys) * D * 2; }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 2)
-kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, int vec) {
+template <typename T, int D, int kTiles>
+__global__ void __launch_bounds__((kSoftWarp + 4 * kTiles) * 32, 3 - kTiles)
+kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_magic, const int vec) {
   constexpr uint32_t kQSlab = kRows * 128, kSlab = kKeys * 128, kQBytes = D / 64 * kQSlab, kTileBytes = D / 64 * kSlab;
-  constexpr uint32_t kCols = 256, kO = 128;            // tensor memory: two buffers of S (and P over it), then O
+  constexpr uint32_t kCols = 256 * kTiles, kO = 128;   // tensor memory of a row tile: two buffers of S (and P over it), then O
   extern __shared__ uint8_t smem_raw[];
-  const uint32_t q_at = (smem_u32(smem_raw) + 1023) & ~1023u, k_at = q_at + kQBytes, v_at = k_at + 2 * kTileBytes;
-  __shared__ Aux aux;
+  const uint32_t q_at = (smem_u32(smem_raw) + 1023) & ~1023u, k_at = q_at + kTiles * kQBytes, v_at = k_at + 2 * kTileBytes;
+  __shared__ Aux<kTiles> aux;
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int head = blockIdx.y, req = blockIdx.z, splits = parts.splits, split = blockIdx.x % splits;
   if (blockIdx.x == 0 && head == 0 && req == 0 && threadIdx.x == 0) parts.plan[kPlanStatus] = kStatusOk;
   const int start = c.starts[req], n_rows = c.starts[req + 1] - start;
-  const int row0 = (int)(gridDim.x / splits - 1 - blockIdx.x / splits) * kRows;    // the rows with the most tokens first
+  const int row0 = (int)(gridDim.x / splits - 1 - blockIdx.x / splits) * (kTiles * kRows);    // the rows with the most tokens first
   if (row0 >= n_rows) return;
   const int bs = c.cache.block_size, ctx = max(0, min(c.seq_lens[req], c.max_blocks * bs));
   const int first = ctx - n_rows + row0;                                 // own position of the CTA's first row
-  const int end = first + min(kRows, n_rows - row0);                     // tokens that its last row attends to, if any
+  const int rows_here = min(kTiles * kRows, n_rows - row0);
+  const int end = first + rows_here;                                     // tokens that its last row attends to, if any
   const int all_tiles = max(0, (end + kKeys - 1) / kKeys), per = (all_tiles + splits - 1) / splits;
   const int tile0 = min(all_tiles, split * per), n_tiles = min(all_tiles, tile0 + per) - tile0;
   const int key0 = tile0 * kKeys;
+  // warps without a row of the request leave the weights to chance: their rows of O are nobody's
+  auto soft_warps = [&](int tile) { return min(4, max(0, rows_here - tile * kRows + 31) / 32); };
   if (threadIdx.x == 0) {
-    mbar_init(&aux.q_full, 4);
+    mbar_init(&aux.q_full, 4 * kTiles);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&aux.k_full[i], 4); mbar_init(&aux.v_full[i], 4); mbar_init(&aux.k_empty[i], 1); mbar_init(&aux.v_empty[i], 1);
-      mbar_init(&aux.s_full[i], 1); mbar_init(&aux.p_full[i], 4);
+      mbar_init(&aux.k_full[i], kGroups); mbar_init(&aux.v_full[i], kGroups); mbar_init(&aux.k_empty[i], 1); mbar_init(&aux.v_empty[i], 1);
+      for (int t = 0; t < kTiles; ++t) {
+        mbar_init(&aux.s_full[t][i], 1); mbar_init(&aux.p_full[t][i], max(1, soft_warps(t))); mbar_init(&aux.o_done[t][i], 1);
+      }
     }
+    for (int i = 0; i < 4; ++i) mbar_init(&aux.scales_full[i], kGroups);
     aux.abort_flag = 0;
     mbar_init_fence();
   }
@@ -106,85 +145,107 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, int vec) {
     if (lane == 0) mbar_arrive_addr(smem_u32(bar));
   };
   bool ok = true;
-  if (warp >= kCopyWarp) {
-    // ---- codes to fp16 ----
-    constexpr int kPieces = D / 16, kAtOnce = 128 / kPieces, kLoads = kKeys / kAtOnce;   // 16-byte pieces of a row, rows at once
-    const int at = threadIdx.x - kCopyWarp * 32, piece = at % kPieces, r0 = at / kPieces;
+  if (warp >= 1 && warp < kSoftWarp) {
+    // ---- codes to fp16, a group of 16 tokens (which never straddles a block) at a time, the warps in turn ----
+    constexpr int kPieces = D / 16, kAtOnce = 32 / kPieces, kLoads = 16 / kAtOnce;   // 16-byte pieces of a row, rows at once
+    struct Group { uint4 k[kLoads], v[kLoads]; float key_scale, value_scale; int rows; };   // rows that count; -1: no block of the cache
+    const int piece = lane % kPieces, r0 = lane / kPieces;
     const int32_t* table = c.tables + (int64_t)req * c.max_blocks;
-    const int64_t row_bytes = (int64_t)c.cache.heads * D, column = (int64_t)head * D + piece * 16;
-    auto store = [&](uint32_t tile, int row, const uint4& codes) {
-      uint32_t h[8];
-      const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        h[2 * i] = e4m3x2_to_f16x2((uint16_t)w[i]);
-        h[2 * i + 1] = e4m3x2_to_f16x2((uint16_t)(w[i] >> 16));
-      }
-      const uint32_t base = tile + piece / 4 * kSlab + row * 128;
-      const int odd = piece / 4 & 1;   // the second slab's pieces in the other order: 8 lanes, 8 different bank groups
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int half = i ^ odd;
-        uint32_t v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = half ? h[4 + e] : h[e];
-        st_shared16(base + (((piece % 4 * 2 + half) ^ (row & 7)) << 4), v);
-      }
+    const int64_t row_bytes = (int64_t)c.cache.heads * D, column = (int64_t)head * D + piece * 16 + r0 * row_bytes;
+    const uint32_t per_block = (uint32_t)bs / 16;
+    const int odd = piece / 4 & 1;   // the second slab's pieces in the other order: 8 lanes, 8 different bank groups
+    const int n_groups = n_tiles * kGroups;
+    auto block_of = [&](int g) {   // of the group's tokens; group / per_block by the high word of a product
+      const uint32_t group = (uint32_t)key0 / 16 + g;
+      return key0 + g * 16 < end ? table[blocks_magic ? __umulhi(group, blocks_magic) : group] : -1;
     };
-    for (int j = 0; j < n_tiles; ++j) {
-      uint4 k[kLoads], v[kLoads];
-      float4 s = make_float4(0.f, -INFINITY, 0.f, 0.f);
+    auto load = [&](Group& f, int g, int block) {
+      const uint32_t group = (uint32_t)key0 / 16 + g, at = blocks_magic ? __umulhi(group, blocks_magic) : group;
+      const bool in = block >= 0 && block < c.cache.num_blocks;
+      f.rows = in ? min(16, end - key0 - g * 16) : -1;
+      if (!in) block = 0;   // something that can be read
+      const int64_t from = block * c.cache.block_stride + (int64_t)((group - at * per_block) * 16) * row_bytes + column;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) f.k[i] = ld_ahead(c.cache.key + from + i * kAtOnce * row_bytes);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) f.v[i] = ld_ahead(c.cache.value + from + i * kAtOnce * row_bytes);
+      f.key_scale = c.cache.key_scale[block * c.cache.scale_stride + head];
+      f.value_scale = c.cache.value_scale[block * c.cache.scale_stride + head];
+    };
+    auto store = [&](uint32_t tile, const uint4 (&codes)[kLoads], int rows_from) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        const int tok = key0 + j * kKeys + r0 + i * kAtOnce;
-        k[i] = v[i] = make_uint4(0, 0, 0, 0);
-        if (tok < end) {
-          const int64_t block = table[tok / bs];
-          if (block >= 0 && block < c.cache.num_blocks) {
-            const int64_t from = block * c.cache.block_stride + tok % bs * row_bytes + column;
-            k[i] = *reinterpret_cast<const uint4*>(c.cache.key + from);
-            v[i] = *reinterpret_cast<const uint4*>(c.cache.value + from);
-          }
-        }
-      }
-      if (at < kGroups) {
-        const int tok = key0 + j * kKeys + at * 16;
-        if (tok < end) {
-          const int64_t block = table[tok / bs];
-          s.x = __int_as_float(0x7fc00000);   // a block outside the cache: the scores of its tokens are NaN
-          if (block >= 0 && block < c.cache.num_blocks) {
-            s.x = c.cache.key_scale[block * c.cache.scale_stride + head];
-            s.y = log2f(c.cache.value_scale[block * c.cache.scale_stride + head]);
-          }
-        }
-      }
-      const int i2 = j & 1;
-      if (j > 1 && !wait(aux.k_empty, j - 2)) { ok = false; break; }
-      if (at < kGroups) aux.scales[j & 3][at] = s;
+        const int row = rows_from + r0 + i * kAtOnce;
+        const uint32_t base = tile + piece / 4 * kSlab + row * 128;
+        const uint4 w = codes[i];
+        const uint32_t half[2][2] = {{odd ? w.z : w.x, odd ? w.w : w.y}, {odd ? w.x : w.z, odd ? w.y : w.w}};
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) store(k_at + i2 * kTileBytes, r0 + i * kAtOnce, k[i]);
+        for (int h = 0; h < 2; ++h) {
+          uint32_t x[4];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            x[2 * e] = e4m3x2_to_f16x2((uint16_t)half[h][e]);
+            x[2 * e + 1] = e4m3x2_to_f16x2((uint16_t)(half[h][e] >> 16));
+          }
+          st_shared16(base + (((piece % 4 * 2 + (h ^ odd)) ^ (row & 7)) << 4), x);
+        }
+      }
+    };
+    auto give = [&](const Group& f, int g) {
+      const int j = g / kGroups, q = g % kGroups, i2 = j & 1;
+      if (j > 1 && !wait(aux.k_empty, j - 2)) return false;
+      if (lane == 0) {
+        // a block outside the cache: the scores of its tokens are NaN (those behind the last one are masked)
+        aux.scales[j & 3][q] = f.rows < 0 ? make_float2(__int_as_float(0x7fc00000), -INFINITY) : make_float2(f.key_scale, log2f(f.value_scale));
+        mbar_arrive_addr(smem_u32(&aux.scales_full[j & 3]));
+      }
+      store(k_at + i2 * kTileBytes, f.k, q * 16);
       arrive(&aux.k_full[i2]);
-      if (j > 1 && !wait(aux.v_empty, j - 2)) { ok = false; break; }
+      if (j > 1 && !wait(aux.v_empty, j - 2)) return false;
+      if (f.rows < 16) {   // rows that do not count have no weight, but zero times whatever they hold might be NaN
+        uint4 v[kLoads];
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) store(v_at + i2 * kTileBytes, r0 + i * kAtOnce, v[i]);
+        for (int i = 0; i < kLoads; ++i) v[i] = r0 + i * kAtOnce < f.rows ? f.v[i] : make_uint4(0, 0, 0, 0);
+        store(v_at + i2 * kTileBytes, v, q * 16);
+      } else {
+        store(v_at + i2 * kTileBytes, f.v, q * 16);
+      }
       arrive(&aux.v_full[i2]);
+      return true;
+    };
+    // two groups in registers: one is on its way while the other is handed over
+    Group a, b;
+    int g = warp - 1, next = block_of(g);
+    if (g < n_groups) load(a, g, next);
+    next = block_of(g + kCopyWarps);
+    for (; g < n_groups && ok; g += 2 * kCopyWarps) {
+      load(b, g + kCopyWarps, next);
+      next = block_of(g + 2 * kCopyWarps);
+      ok = give(a, g);
+      if (g + kCopyWarps >= n_groups || !ok) break;
+      load(a, g + 2 * kCopyWarps, next);
+      next = block_of(g + 3 * kCopyWarps);
+      ok = give(b, g + kCopyWarps);
     }
   } else if (warp == 0) {
     // ---- products ----
     constexpr uint32_t s_idesc = mma_idesc(0, 128, kKeys, false);
     constexpr uint32_t o_idesc = mma_idesc(0, 128, D, false) | (1u << 16);   // B is MN-major
-    auto scores = [&](int j) {   // S of tile j
+    auto scores = [&](int j) {   // S of key tile j
       const int i = j & 1;
-      // the buffer still holds the weights of tile j - 2
+      // the buffers still hold the weights of tile j - 2
       if (!wait(aux.k_full, j) || (j > 1 && !wait(aux.v_empty, j - 2))) return false;
       tc_fence_after();
       if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          tc_mma_cta(tmem + i * kKeys, desc_lo(q_at + k / 4 * kQSlab + k % 4 * 32, 16), desc_hi(1024, true),
-                     desc_lo(k_at + i * kTileBytes + k / 4 * kSlab + k % 4 * 32, 16), desc_hi(1024, true), s_idesc, k != 0);
+        for (int t = 0; t < kTiles; ++t) {
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            tc_mma_cta(tmem + t * 256 + i * kKeys, desc_lo(q_at + t * kQBytes + k / 4 * kQSlab + k % 4 * 32, 16), desc_hi(1024, true),
+                       desc_lo(k_at + i * kTileBytes + k / 4 * kSlab + k % 4 * 32, 16), desc_hi(1024, true), s_idesc, k != 0);
+          tc_commit_cta(smem_u32(&aux.s_full[t][i]));
+        }
         tc_commit_cta(smem_u32(&aux.k_empty[i]));
-        tc_commit_cta(smem_u32(&aux.s_full[i]));
       }
       __syncwarp();
       return true;
@@ -193,23 +254,33 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, int vec) {
       ok = mbar_wait_warp(smem_u32(&aux.q_full), 0, abort_flag, status, kStatusTileWait, lane) && scores(0);
     for (int j = 0; j < n_tiles && ok; ++j) {
       const int i = j & 1;
-      if ((j + 1 < n_tiles && !scores(j + 1)) || !wait(aux.v_full, j) || !wait(aux.p_full, j)) { ok = false; break; }
-      tc_fence_after();
-      if (elect_one()) {
+      if ((j + 1 < n_tiles && !scores(j + 1)) || !wait(aux.v_full, j)) { ok = false; break; }
 #pragma unroll
-        for (int k = 0; k < kKeys / 16; ++k)
-          mma_tmem_a(tmem + kO, tmem + i * kKeys + k * 8, desc_lo(v_at + i * kTileBytes + k * 2048, kSlab), desc_hi(1024, true), o_idesc,
-                     j > 0 || k != 0);
-        tc_commit_cta(smem_u32(&aux.v_empty[i]));
+      for (int t = 0; t < kTiles; ++t) {
+        if (soft_warps(t) > 0) {
+          if (!wait(aux.p_full[t], j)) { ok = false; break; }
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < kKeys / 16; ++k)
+              mma_tmem_a(tmem + t * 256 + kO, tmem + t * 256 + i * kKeys + k * 8, desc_lo(v_at + i * kTileBytes + k * 2048, kSlab),
+                         desc_hi(1024, true), o_idesc, j > 0 || k != 0);
+            tc_commit_cta(smem_u32(&aux.o_done[t][i]));
+          }
+          __syncwarp();
+        }
       }
+      if (!ok) break;
+      if (elect_one()) tc_commit_cta(smem_u32(&aux.v_empty[i]));
       __syncwarp();
     }
   } else {
     // ---- softmax: a thread per row; the warp's quarter of tensor memory is its number modulo 4 ----
-    const int quarter = warp & 3, row = quarter * 32 + lane;
-    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16), o_at = lanes + kO;
+    const int tile = (warp - kSoftWarp) / 4, quarter = warp & 3, row = tile * kRows + quarter * 32 + lane;
+    const uint32_t lanes = tmem + tile * 256 + ((uint32_t)(quarter * 32) << 16), o_at = lanes + kO;
     const int64_t t = (int64_t)start + row0 + row;
-    const bool mine = row0 + row < n_rows && t >= 0 && t < c.rows;
+    const bool mine = row < rows_here && t >= 0 && t < c.rows;
+    const bool live = quarter < soft_warps(tile);
     float up = 1.f;   // what the row's scores are multiplied by for its query's fp16 form
     {
       const T* src = static_cast<const T*>(c.query) + (mine ? t : 0) * c.query_stride + (int64_t)head * D;
@@ -247,37 +318,50 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, int vec) {
         uint32_t w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = half2_bits(x[2 * i] * down, x[2 * i + 1] * down);
-        st_shared16(q_at + e / 64 * kQSlab + row * 128 + (((e / 8 & 7) ^ (row & 7)) << 4), w);
+        st_shared16(q_at + tile * kQBytes + e / 64 * kQSlab + (row % kRows) * 128 + (((e / 8 & 7) ^ (row & 7)) << 4), w);
       }
       arrive(&aux.q_full);
     }
     const float coef = parts.scale_log2 * up;
     float m = -INFINITY, l = 0.f, ref = -INFINITY;
-    for (int j = 0; j < n_tiles; ++j) {
+    for (int j = 0; j < n_tiles && live; ++j) {
       const uint32_t s_at = lanes + (j & 1) * kKeys;
-      const int seen = first + row - key0 - j * kKeys;   // the last token of the tile that the row attends to
-      const bool diagonal = key0 + j * kKeys + kKeys - 1 > first;
-      if (!wait(aux.s_full, j) || !wait(aux.v_full, j)) { ok = false; break; }   // the scales are written before V
+      const int seen = first + row - key0 - j * kKeys;   // the last token of the key tile that the row attends to
+      if (!wait(aux.s_full[tile], j) ||
+          !mbar_wait_warp(smem_u32(&aux.scales_full[j & 3]), (uint32_t)(j >> 2) & 1u, abort_flag, status, kStatusTileWait, lane)) {
+        ok = false;
+        break;
+      }
       tc_fence_after();
       uint32_t v[kKeys];
       tmem_ld32(s_at, v);
       tmem_ld32(s_at + 32, v + 32);
-      tmem_ld_wait();
-      if (diagonal) {
-#pragma unroll
-        for (int i = 0; i < kKeys; ++i)
-          if (i > seen) v[i] = 0xff800000u;   // -infinity
-      }
-      float by[kGroups], lv[kGroups], m_new = m, r_new = -INFINITY;
+      float by[kGroups], lv[kGroups];
 #pragma unroll
       for (int b = 0; b < kGroups; ++b) {
-        const float4 s = aux.scales[j & 3][b];
+        const float2 s = aux.scales[j & 3][b];
         by[b] = coef * s.x;
         lv[b] = s.y;
+      }
+      tmem_ld_wait();
+      if (key0 + j * kKeys + kKeys - 1 > first + tile * kRows) {   // the tile meets the diagonal
+#pragma unroll
+        for (int b = 0; b < kGroups; ++b) {
+          // -infinity times a factor that is 0 or NaN would be NaN: such a factor goes into the scores
+          const bool plain = by[b] > 0.f;
+          const uint32_t fill = by[b] == 0.f ? 0u : 0x7fc00000u;
+          if (!plain) by[b] = 1.f;
+#pragma unroll
+          for (int i = 16 * b; i < 16 * b + 16; ++i) v[i] = i > seen ? 0xff800000u : plain ? v[i] : fill;
+        }
+      }
+      float m_new = m, r_new = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < kGroups; ++b) {
         float tops[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 16; ++i) tops[i & 1] = fmaxf(tops[i & 1], __uint_as_float(v[16 * b + i]));
-        const float top = fmaxf(tops[0], tops[1]) * by[b];   // NaN (-infinity times a scale of 0) counts as none
+        for (int i = 0; i < 16; i += 2) tops[i / 2 & 1] = max3(tops[i / 2 & 1], __uint_as_float(v[16 * b + i]), __uint_as_float(v[16 * b + i + 1]));
+        const float top = fmaxf(tops[0], tops[1]) * by[b];   // NaN counts as none
         m_new = fmaxf(m_new, top);
         r_new = fmaxf(r_new, top + lv[b]);
       }
@@ -286,11 +370,11 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, int vec) {
       } else {
         const bool move = r_new > ref && !(r_new - ref <= kSlack);
         if (__any_sync(0xffffffffu, move)) {
-          if (!wait(aux.v_empty, j - 1)) { ok = false; break; }   // O is as the last tile left it
+          if (!wait(aux.o_done[tile], j - 1)) { ok = false; break; }   // O is as the last tile left it
           tc_fence_after();
           const float down = move && ref != -INFINITY ? ex2(ref - r_new) : 1.f;
           if (move) ref = r_new;
-#pragma unroll
+#pragma unroll 1
           for (int d = 0; d < D; d += 16) {
             uint32_t o[16];
             tmem_ld16(o_at + d, o);
@@ -304,31 +388,29 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, int vec) {
       const float shift = m_new == -INFINITY ? 0.f : m_new, base = shift - (ref == -INFINITY ? 0.f : ref) + kUp;
       l *= m == -INFINITY ? 0.f : ex2(m - shift);
       m = m_new;
-      float sums[2] = {0.f, 0.f};
+      // the weights as they meet V, 2^(x + off): their sums go back to the scores' own reference block by block.  A block whose off is
+      // below -60 has no weight in fp16 either way
 #pragma unroll
       for (int b = 0; b < kGroups; ++b) {
-        const float gain = ex2(fminf(base + lv[b], 126.f));
+        const float off = base + lv[b] < -60.f ? -60.f : base + lv[b], from = off - shift;
+        float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int i = 16 * b; i < 16 * b + 16; i += 2) {
-          float x = fmaf(__uint_as_float(v[i]), by[b], -shift), y = fmaf(__uint_as_float(v[i + 1]), by[b], -shift);
-          if (diagonal) {   // -infinity times a scale that is 0 or NaN is not
-            x = i > seen ? -INFINITY : x;
-            y = i + 1 > seen ? -INFINITY : y;
-          }
-          x = ex2(x);
-          y = ex2(y);
-          sums[0] += x;
-          sums[1] += y;
-          v[i / 2] = half2_bits(x * gain, y * gain);
+          float2 x = fma2(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), by[b], from);
+          x.x = ex2(x.x);
+          x.y = ex2(x.y);
+          sums[i / 2 & 1] = add2(sums[i / 2 & 1], x);
+          v[i / 2] = half2_bits(x.x, x.y);
         }
+        sums[0] = add2(sums[0], sums[1]);
+        l = fmaf(sums[0].x + sums[0].y, ex2(-off), l);
       }
-      l += sums[0] + sums[1];
       tmem_st16(s_at, v);
       tmem_st16(s_at + 16, v + 16);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_addr(smem_u32(&aux.p_full[j & 1]));
+      if (lane == 0) mbar_arrive_addr(smem_u32(&aux.p_full[tile][j & 1]));
     }
     ok = ok && (n_tiles == 0 || wait(aux.v_empty, n_tiles - 1));
     tc_fence_after();
@@ -380,22 +462,32 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, int vec) {
   if (warp == 0) { tc_fence_after(); tmem_free(tmem, kCols); }
 }
 
-template <typename T, int D>
+template <typename T, int D, int kTiles>
 int launch(const Kv8Call& c, const Kv8Parts& parts, cudaStream_t stream) {
   static bool done[64] = {false};
-  auto kernel = kv8_tile_kernel<T, D>;
+  auto kernel = kv8_tile_kernel<T, D, kTiles>;
+  constexpr size_t smem = tile_smem<D, kTiles>();
   int dev = 0;
   APS_CUDA(cudaGetDevice(&dev));
   APS_REQUIRE(dev >= 0 && dev < 64, APS_ERR_CUDA, "device index %d out of range", dev);
   if (!done[dev]) {
-    APS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tile_smem<D>()));
+    APS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     APS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
     done[dev] = true;
   }
   const int vec = aligned_to(c.query, 16) && aligned_to(c.out, 16) && c.query_stride % 8 == 0 && c.out_stride % 8 == 0;
-  const int blocks = (c.max_rows + kRows - 1) / kRows;
-  kernel<<<dim3(blocks * parts.splits, c.cache.heads, c.batch), kThreads, tile_smem<D>(), stream>>>(c, parts, vec);
+  const int blocks = (c.max_rows + kTiles * kRows - 1) / (kTiles * kRows);
+  // x / n = high word of x * ceil(2^32 / n), exact for x below 2^26 and n up to 64
+  const uint32_t n = c.cache.block_size / 16, magic = n == 1 ? 0u : (uint32_t)(((uint64_t(1) << 32) + n - 1) / n);
+  kernel<<<dim3(blocks * parts.splits, c.cache.heads, c.batch), (kSoftWarp + 4 * kTiles) * 32, smem, stream>>>(c, parts, magic, vec);
   return launch_status("kv8_tile_kernel");
+}
+
+template <typename T>
+int launch_typed(const Kv8Call& c, const Kv8Parts& parts, cudaStream_t stream) {
+  const bool two = c.max_rows > kRows;
+  if (c.cache.head_size == 128) return two ? launch<T, 128, 2>(c, parts, stream) : launch<T, 128, 1>(c, parts, stream);
+  return two ? launch<T, 64, 2>(c, parts, stream) : launch<T, 64, 1>(c, parts, stream);
 }
 
 }  // namespace
@@ -403,7 +495,7 @@ int launch(const Kv8Call& c, const Kv8Parts& parts, cudaStream_t stream) {
 bool kv8_tiles_take(const Kv8Call& c) {
   // the maximum is taken of the raw scores: a scale that is not positive would need their minimum
   return c.starts != nullptr && c.max_rows > 1 && (c.dtype == APS_F16 || c.dtype == APS_BF16) &&
-         (c.cache.head_size == 64 || c.cache.head_size == 128) && c.scale >= 1.17549435e-38f && c.scale < 1.70141183e38f && c.batch <= 65535;
+         (c.cache.head_size == 64 || c.cache.head_size == 128) && c.cache.num_blocks > 0 && c.scale >= 1.17549435e-38f && c.scale < 1.70141183e38f && c.batch <= 65535;
 }
 
 // Parts that the tokens of a tile of rows are cut into: enough CTAs for two per SM, four key tiles each at least.
@@ -416,9 +508,7 @@ int kv8_tile_splits(const Kv8Call& c) {
 }
 
 int launch_kv8_tiles(const Kv8Call& c, const Kv8Parts& parts, cudaStream_t stream) {
-  if (c.dtype == APS_BF16)
-    return c.cache.head_size == 128 ? launch<__nv_bfloat16, 128>(c, parts, stream) : launch<__nv_bfloat16, 64>(c, parts, stream);
-  return c.cache.head_size == 128 ? launch<__half, 128>(c, parts, stream) : launch<__half, 64>(c, parts, stream);
+  return c.dtype == APS_BF16 ? launch_typed<__nv_bfloat16>(c, parts, stream) : launch_typed<__half>(c, parts, stream);
 }
 
 }  // namespace aps
