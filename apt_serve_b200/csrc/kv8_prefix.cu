@@ -231,6 +231,8 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_mag
     // ---- products ----
     constexpr uint32_t s_idesc = mma_idesc(0, 128, kKeys, false);
     constexpr uint32_t o_idesc = mma_idesc(0, 128, D, false) | (1u << 16);   // B is MN-major
+    // descriptors' low halves: an offset in shared memory adds its sixteenth
+    const uint32_t q_lo = desc_lo(q_at, 16), k_lo = desc_lo(k_at, 16), v_lo = desc_lo(v_at, kSlab);
     auto scores = [&](int j) {   // S of key tile j
       const int i = j & 1;
       // the buffers still hold the weights of tile j - 2
@@ -241,8 +243,8 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_mag
         for (int t = 0; t < kTiles; ++t) {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
-            tc_mma_cta(tmem + t * 256 + i * kKeys, desc_lo(q_at + t * kQBytes + k / 4 * kQSlab + k % 4 * 32, 16), desc_hi(1024, true),
-                       desc_lo(k_at + i * kTileBytes + k / 4 * kSlab + k % 4 * 32, 16), desc_hi(1024, true), s_idesc, k != 0);
+            tc_mma_cta(tmem + t * 256 + i * kKeys, q_lo + (t * kQBytes + k / 4 * kQSlab + k % 4 * 32) / 16, desc_hi(1024, true),
+                       k_lo + i * (kTileBytes / 16) + (k / 4 * kSlab + k % 4 * 32) / 16, desc_hi(1024, true), s_idesc, k != 0);
           tc_commit_cta(smem_u32(&aux.s_full[t][i]));
         }
         tc_commit_cta(smem_u32(&aux.k_empty[i]));
@@ -263,7 +265,7 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_mag
           if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < kKeys / 16; ++k)
-              mma_tmem_a(tmem + t * 256 + kO, tmem + t * 256 + i * kKeys + k * 8, desc_lo(v_at + i * kTileBytes + k * 2048, kSlab),
+              mma_tmem_a(tmem + t * 256 + kO, tmem + t * 256 + i * kKeys + k * 8, v_lo + i * (kTileBytes / 16) + k * 128,
                          desc_hi(1024, true), o_idesc, j > 0 || k != 0);
             tc_commit_cta(smem_u32(&aux.o_done[t][i]));
           }
@@ -284,42 +286,47 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_mag
     float up = 1.f;   // what the row's scores are multiplied by for its query's fp16 form
     {
       const T* src = static_cast<const T*>(c.query) + (mine ? t : 0) * c.query_stride + (int64_t)head * D;
-      auto eight = [&](int e, float* x) {
-        if (!mine) {
+      uint4 q[D / 8];   // the whole row at once: one round trip
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = 0.f;
-        } else if (vec) {
-          Vec16<T>::unpack(*reinterpret_cast<const uint4*>(src + e), x);
-        } else {
+      for (int e = 0; e < D / 8; ++e) q[e] = make_uint4(0, 0, 0, 0);
+      if (mine && vec) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = Elem<T>::to_float(src[e + i]);
+        for (int e = 0; e < D / 8; ++e) q[e] = ld_ahead(reinterpret_cast<const uint8_t*>(src + 8 * e));
+      } else if (mine) {
+#pragma unroll
+        for (int e = 0; e < D / 8; ++e) {
+          struct alignas(16) { T x[8]; } some;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) some.x[i] = src[8 * e + i];
+          q[e] = *reinterpret_cast<const uint4*>(&some);
         }
-      };
-      float down = 1.f;
-      if (std::is_same<T, __nv_bfloat16>::value) {
+      }
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
         float top = 0.f;
-#pragma unroll 2
-        for (int e = 0; e < D; e += 8) {
+#pragma unroll
+        for (int e = 0; e < D / 8; ++e) {
           float x[8];
-          eight(e, x);
+          Vec16<T>::unpack(q[e], x);
 #pragma unroll
           for (int i = 0; i < 8; ++i)
             if (fabsf(x[i]) <= 3.402823466e38f) top = fmaxf(top, fabsf(x[i]));
         }
         // the largest element to 2^14 ... 2^15; factors within fp32's normal range
         const int p = min(120, 127 + 14 - (int)(__float_as_uint(top) >> 23));
-        down = __uint_as_float((uint32_t)(127 + p) << 23);
+        const float down = __uint_as_float((uint32_t)(127 + p) << 23);
         up = __uint_as_float((uint32_t)(127 - p) << 23);
-      }
-#pragma unroll 2
-      for (int e = 0; e < D; e += 8) {
-        float x[8];
-        eight(e, x);
-        uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = half2_bits(x[2 * i] * down, x[2 * i + 1] * down);
-        st_shared16(q_at + tile * kQBytes + e / 64 * kQSlab + (row % kRows) * 128 + (((e / 8 & 7) ^ (row & 7)) << 4), w);
+        for (int e = 0; e < D / 8; ++e) {
+          float x[8];
+          Vec16<T>::unpack(q[e], x);
+          q[e] = make_uint4(half2_bits(x[0] * down, x[1] * down), half2_bits(x[2] * down, x[3] * down),
+                            half2_bits(x[4] * down, x[5] * down), half2_bits(x[6] * down, x[7] * down));
+        }
       }
+#pragma unroll
+      for (int e = 0; e < D / 8; ++e)
+        st_shared16(q_at + tile * kQBytes + e / 8 * kQSlab + (row % kRows) * 128 + (((e & 7) ^ (row & 7)) << 4),
+                    reinterpret_cast<const uint32_t*>(&q[e]));
       arrive(&aux.q_full);
     }
     const float coef = parts.scale_log2 * up;
