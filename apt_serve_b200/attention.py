@@ -46,6 +46,7 @@ def _scratch_of(device: torch.device, need: int) -> Tuple[torch.Tensor, int]:
     ws = _workspaces.get(device)
     if ws is None or ws.numel() < need:
         ws = torch.empty(need, dtype=torch.uint8, device=device)
+        ws[:256].zero_()   # no call has left a status in it (a cache write that takes scratch leaves none)
         _workspaces[device] = ws
     return ws, need
 

@@ -53,6 +53,11 @@ __device__ __forceinline__ uint16_t float2_to_e4m3x2(float lo, float hi) {
 __device__ __forceinline__ uint32_t float4_to_e4m3x4(const float* f) {
   return (uint32_t)float2_to_e4m3x2(f[0], f[1]) | (uint32_t)float2_to_e4m3x2(f[2], f[3]) << 16;
 }
+__device__ __forceinline__ uint16_t f16x2_to_e4m3x2(uint32_t halves) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(halves));
+  return r;
+}
 // The smallest power of two s >= 2^-118 with top <= 448 s (448 = 1.75 * 2^8; top finite and not negative).
 __device__ __forceinline__ float e4m3_scale(float top) {
   const uint32_t u = __float_as_uint(top);

@@ -19,7 +19,8 @@
 namespace aps {
 namespace {
 
-constexpr int kRows = 128, kKeys = 64, kGroups = kKeys / 16, kCopyWarps = 4, kSoftWarp = 1 + kCopyWarps;
+constexpr int kRows = 128, kCopyWarps = 4, kSoftWarp = 1 + kCopyWarps;
+constexpr int kKeys = 64, kGroups = kKeys / 16;
 constexpr float kSlack = 8.f;   // log2 of how much R may have grown before O is rescaled
 constexpr float kUp = 7.f;      // log2 of what the weights are kept at: 2^15 at most
 constexpr int kStatusTileWait = 6;
@@ -30,7 +31,7 @@ struct Aux {
   // key tile j: entry j & 1, phase j >> 1
   uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[kTiles][2], p_full[kTiles][2], o_done[kTiles][2];
   uint64_t scales_full[4];        // entry j & 3, phase j >> 2: written again only after the weights of tile j + 1
-  float2 scales[4][kGroups];      // key scale, log2 of the value scale
+  float2 scales[4][kKeys / 16];   // key scale, log2 of the value scale
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -48,6 +49,15 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
       "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
       ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
       "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+// tmem_ld32's registers may be read behind this.
+__device__ __forceinline__ void tmem_ld_wait32(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+      : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+      "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
+      "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
+      "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+      :: "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
@@ -92,13 +102,13 @@ __device__ __forceinline__ void st_shared16(uint32_t addr, const uint32_t* w) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
 }
 
-template <int D, int kTiles> constexpr size_t tile_smem() { return 1024 + (size_t)(kTiles * kRows + 4 * kKeys) * D * 2; }
+template <int D, int kTiles> __host__ __device__ constexpr size_t tile_smem() { return 1024 + (size_t)(kTiles * kRows + 4 * kKeys) * D * 2; }
 
 template <typename T, int D, int kTiles>
-__global__ void __launch_bounds__((kSoftWarp + 4 * kTiles) * 32, 3 - kTiles)
+__global__ void __launch_bounds__((kSoftWarp + 4 * kTiles) * 32, kTiles == 1 ? 2 : 1)
 kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_magic, const int vec) {
   constexpr uint32_t kQSlab = kRows * 128, kSlab = kKeys * 128, kQBytes = D / 64 * kQSlab, kTileBytes = D / 64 * kSlab;
-  constexpr uint32_t kCols = 256 * kTiles, kO = 128;   // tensor memory of a row tile: two buffers of S (and P over it), then O
+  constexpr uint32_t kCols = 256 * kTiles, kO = 128;   // tensor memory of a row tile: S (and P over it), then O
   extern __shared__ uint8_t smem_raw[];
   const uint32_t q_at = (smem_u32(smem_raw) + 1023) & ~1023u, k_at = q_at + kTiles * kQBytes, v_at = k_at + 2 * kTileBytes;
   __shared__ Aux<kTiles> aux;
@@ -120,12 +130,12 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_mag
   if (threadIdx.x == 0) {
     mbar_init(&aux.q_full, 4 * kTiles);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&aux.k_full[i], kGroups); mbar_init(&aux.v_full[i], kGroups); mbar_init(&aux.k_empty[i], 1); mbar_init(&aux.v_empty[i], 1);
+      mbar_init(&aux.k_full[i], kCopyWarps); mbar_init(&aux.v_full[i], kCopyWarps); mbar_init(&aux.k_empty[i], 1); mbar_init(&aux.v_empty[i], 1);
       for (int t = 0; t < kTiles; ++t) {
         mbar_init(&aux.s_full[t][i], 1); mbar_init(&aux.p_full[t][i], max(1, soft_warps(t))); mbar_init(&aux.o_done[t][i], 1);
       }
     }
-    for (int i = 0; i < 4; ++i) mbar_init(&aux.scales_full[i], kGroups);
+    for (int i = 0; i < 4; ++i) mbar_init(&aux.scales_full[i], kCopyWarps);
     aux.abort_flag = 0;
     mbar_init_fence();
   }
@@ -146,31 +156,32 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_mag
   };
   bool ok = true;
   if (warp >= 1 && warp < kSoftWarp) {
-    // ---- codes to fp16, a group of 16 tokens (which never straddles a block) at a time, the warps in turn ----
+    // ---- codes to fp16: every warp its groups of 16 tokens (which never straddle a block) of a key tile ----
     constexpr int kPieces = D / 16, kAtOnce = 32 / kPieces, kLoads = 16 / kAtOnce;   // 16-byte pieces of a row, rows at once
-    struct Group { uint4 k[kLoads], v[kLoads]; float key_scale, value_scale; int rows; };   // rows that count; -1: no block of the cache
+    constexpr int kMine = kGroups / kCopyWarps;
     const int piece = lane % kPieces, r0 = lane / kPieces;
     const int32_t* table = c.tables + (int64_t)req * c.max_blocks;
     const int64_t row_bytes = (int64_t)c.cache.heads * D, column = (int64_t)head * D + piece * 16 + r0 * row_bytes;
     const uint32_t per_block = (uint32_t)bs / 16;
     const int odd = piece / 4 & 1;   // the second slab's pieces in the other order: 8 lanes, 8 different bank groups
-    const int n_groups = n_tiles * kGroups;
+    const int mine = warp - 1;
+    struct Place { int64_t from; int block, rows; };   // rows that count; none: no block of the cache, or behind the last token
     auto block_of = [&](int g) {   // of the group's tokens; group / per_block by the high word of a product
       const uint32_t group = (uint32_t)key0 / 16 + g;
       return key0 + g * 16 < end ? table[blocks_magic ? __umulhi(group, blocks_magic) : group] : -1;
     };
-    auto load = [&](Group& f, int g, int block) {
+    auto place = [&](int g, int block) {
       const uint32_t group = (uint32_t)key0 / 16 + g, at = blocks_magic ? __umulhi(group, blocks_magic) : group;
+      Place p;
       const bool in = block >= 0 && block < c.cache.num_blocks;
-      f.rows = in ? min(16, end - key0 - g * 16) : -1;
-      if (!in) block = 0;   // something that can be read
-      const int64_t from = block * c.cache.block_stride + (int64_t)((group - at * per_block) * 16) * row_bytes + column;
+      p.rows = in ? min(16, end - key0 - g * 16) : -1;
+      p.block = in ? block : 0;   // something that can be read
+      p.from = p.block * c.cache.block_stride + (int64_t)((group - at * per_block) * 16) * row_bytes + column;
+      return p;
+    };
+    auto load = [&](uint4 (&codes)[kLoads], const uint8_t* cache, const Place& p) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) f.k[i] = ld_ahead(c.cache.key + from + i * kAtOnce * row_bytes);
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) f.v[i] = ld_ahead(c.cache.value + from + i * kAtOnce * row_bytes);
-      f.key_scale = c.cache.key_scale[block * c.cache.scale_stride + head];
-      f.value_scale = c.cache.value_scale[block * c.cache.scale_stride + head];
+      for (int i = 0; i < kLoads; ++i) codes[i] = ld_ahead(cache + p.from + i * kAtOnce * row_bytes);
     };
     auto store = [&](uint32_t tile, const uint4 (&codes)[kLoads], int rows_from) {
 #pragma unroll
@@ -191,41 +202,54 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_mag
         }
       }
     };
-    auto give = [&](const Group& f, int g) {
-      const int j = g / kGroups, q = g % kGroups, i2 = j & 1;
-      if (j > 1 && !wait(aux.k_empty, j - 2)) return false;
-      if (lane == 0) {
-        // a block outside the cache: the scores of its tokens are NaN (those behind the last one are masked)
-        aux.scales[j & 3][q] = f.rows < 0 ? make_float2(__int_as_float(0x7fc00000), -INFINITY) : make_float2(f.key_scale, log2f(f.value_scale));
-        mbar_arrive_addr(smem_u32(&aux.scales_full[j & 3]));
-      }
-      store(k_at + i2 * kTileBytes, f.k, q * 16);
-      arrive(&aux.k_full[i2]);
-      if (j > 1 && !wait(aux.v_empty, j - 2)) return false;
-      if (f.rows < 16) {   // rows that do not count have no weight, but zero times whatever they hold might be NaN
-        uint4 v[kLoads];
+    // a tile's codes are on their way while the last one's are handed over; the table's entries one tile further ahead
+    uint4 k[kMine][kLoads], v[kMine][kLoads];
+    Place now[kMine];
+    int next[kMine];
+    float2 scale[kMine];
+    auto load_scale = [&](const Place& p) {
+      const int64_t at = p.block * c.cache.scale_stride + head;
+      return make_float2(c.cache.key_scale[at], c.cache.value_scale[at]);
+    };
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) v[i] = r0 + i * kAtOnce < f.rows ? f.v[i] : make_uint4(0, 0, 0, 0);
-        store(v_at + i2 * kTileBytes, v, q * 16);
-      } else {
-        store(v_at + i2 * kTileBytes, f.v, q * 16);
+    for (int i = 0; i < kMine; ++i) {
+      now[i] = place(mine + i * kCopyWarps, n_tiles > 0 ? block_of(mine + i * kCopyWarps) : -1);
+      load(k[i], c.cache.key, now[i]);
+      scale[i] = load_scale(now[i]);
+      load(v[i], c.cache.value, now[i]);
+      next[i] = n_tiles > 1 ? block_of(kGroups + mine + i * kCopyWarps) : -1;
+    }
+    for (int j = 0; j < n_tiles; ++j) {
+      const int i2 = j & 1;
+      Place then[kMine];
+      if (j > 1 && !wait(aux.k_empty, j - 2)) { ok = false; break; }
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int q = mine + i * kCopyWarps;
+        if (lane == 0)   // a block outside the cache: the scores of its tokens are NaN (those behind the last one are masked)
+          aux.scales[j & 3][q] = now[i].rows < 0 ? make_float2(__int_as_float(0x7fc00000), -INFINITY) : make_float2(scale[i].x, log2f(scale[i].y));
+        store(k_at + i2 * kTileBytes, k[i], q * 16);
+        then[i] = place((j + 1) * kGroups + q, next[i]);
+        load(k[i], c.cache.key, then[i]);
+        scale[i] = load_scale(then[i]);
+        next[i] = j + 2 < n_tiles ? block_of((j + 2) * kGroups + q) : -1;
+      }
+      if (lane == 0) mbar_arrive_addr(smem_u32(&aux.scales_full[j & 3]));
+      arrive(&aux.k_full[i2]);
+      if (j > 1 && !wait(aux.v_empty, j - 2)) { ok = false; break; }
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int q = mine + i * kCopyWarps;
+        if (now[i].rows < 16) {   // rows that do not count have no weight, but zero times whatever they hold might be NaN
+#pragma unroll
+          for (int e = 0; e < kLoads; ++e)
+            if (r0 + e * kAtOnce >= now[i].rows) v[i][e] = make_uint4(0, 0, 0, 0);
+        }
+        store(v_at + i2 * kTileBytes, v[i], q * 16);
+        load(v[i], c.cache.value, then[i]);
+        now[i] = then[i];
       }
       arrive(&aux.v_full[i2]);
-      return true;
-    };
-    // two groups in registers: one is on its way while the other is handed over
-    Group a, b;
-    int g = warp - 1, next = block_of(g);
-    if (g < n_groups) load(a, g, next);
-    next = block_of(g + kCopyWarps);
-    for (; g < n_groups && ok; g += 2 * kCopyWarps) {
-      load(b, g + kCopyWarps, next);
-      next = block_of(g + 2 * kCopyWarps);
-      ok = give(a, g);
-      if (g + kCopyWarps >= n_groups || !ok) break;
-      load(a, g + 2 * kCopyWarps, next);
-      next = block_of(g + 3 * kCopyWarps);
-      ok = give(b, g + kCopyWarps);
     }
   } else if (warp == 0) {
     // ---- products ----
@@ -233,48 +257,57 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_mag
     constexpr uint32_t o_idesc = mma_idesc(0, 128, D, false) | (1u << 16);   // B is MN-major
     // descriptors' low halves: an offset in shared memory adds its sixteenth
     const uint32_t q_lo = desc_lo(q_at, 16), k_lo = desc_lo(k_at, 16), v_lo = desc_lo(v_at, kSlab);
-    auto scores = [&](int j) {   // S of key tile j
-      const int i = j & 1;
-      // the buffers still hold the weights of tile j - 2
-      if (!wait(aux.k_full, j) || (j > 1 && !wait(aux.v_empty, j - 2))) return false;
-      tc_fence_after();
+    auto scores = [&](int t, int j) {   // S of row tile t and key tile j
       if (elect_one()) {
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            tc_mma_cta(tmem + t * 256 + i * kKeys, q_lo + (t * kQBytes + k / 4 * kQSlab + k % 4 * 32) / 16, desc_hi(1024, true),
-                       k_lo + i * (kTileBytes / 16) + (k / 4 * kSlab + k % 4 * 32) / 16, desc_hi(1024, true), s_idesc, k != 0);
-          tc_commit_cta(smem_u32(&aux.s_full[t][i]));
-        }
-        tc_commit_cta(smem_u32(&aux.k_empty[i]));
+        for (int k = 0; k < D / 16; ++k)
+          tc_mma_cta(tmem + t * 256 + (j & 1) * kKeys, q_lo + (t * kQBytes + k / 4 * kQSlab + k % 4 * 32) / 16, desc_hi(1024, true),
+                     k_lo + (j & 1) * (kTileBytes / 16) + (k / 4 * kSlab + k % 4 * 32) / 16, desc_hi(1024, true), s_idesc, k != 0);
+        tc_commit_cta(smem_u32(&aux.s_full[t][(j & 1)]));
+        if (t == kTiles - 1) tc_commit_cta(smem_u32(&aux.k_empty[j & 1]));
       }
       __syncwarp();
-      return true;
     };
-    if (n_tiles > 0)
-      ok = mbar_wait_warp(smem_u32(&aux.q_full), 0, abort_flag, status, kStatusTileWait, lane) && scores(0);
-    for (int j = 0; j < n_tiles && ok; ++j) {
-      const int i = j & 1;
-      if ((j + 1 < n_tiles && !scores(j + 1)) || !wait(aux.v_full, j)) { ok = false; break; }
+    auto values = [&](int t, int j) {
+      if (elect_one()) {
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-        if (soft_warps(t) > 0) {
-          if (!wait(aux.p_full[t], j)) { ok = false; break; }
-          tc_fence_after();
-          if (elect_one()) {
-#pragma unroll
-            for (int k = 0; k < kKeys / 16; ++k)
-              mma_tmem_a(tmem + t * 256 + kO, tmem + t * 256 + i * kKeys + k * 8, v_lo + i * (kTileBytes / 16) + k * 128,
-                         desc_hi(1024, true), o_idesc, j > 0 || k != 0);
-            tc_commit_cta(smem_u32(&aux.o_done[t][i]));
-          }
-          __syncwarp();
-        }
+        for (int k = 0; k < kKeys / 16; ++k)
+          mma_tmem_a(tmem + t * 256 + kO, tmem + t * 256 + (j & 1) * kKeys + k * 8, v_lo + (j & 1) * (kTileBytes / 16) + k * 128,
+                     desc_hi(1024, true), o_idesc, j > 0 || k != 0);
+        tc_commit_cta(smem_u32(&aux.o_done[t][(j & 1)]));
+        if (t == kTiles - 1) tc_commit_cta(smem_u32(&aux.v_empty[j & 1]));
       }
-      if (!ok) break;
-      if (elect_one()) tc_commit_cta(smem_u32(&aux.v_empty[i]));
       __syncwarp();
+    };
+    const bool second = kTiles == 2 && soft_warps(1) > 0;
+    if (n_tiles > 0) {
+      ok = mbar_wait_warp(smem_u32(&aux.q_full), 0, abort_flag, status, kStatusTileWait, lane) && wait(aux.k_full, 0);
+      tc_fence_after();
+      if (ok) scores(0, 0);
+      if constexpr (kTiles == 2) {
+        // the second row tile half a turn behind the first: one's exponentials run beside the other's maxima and waits
+        ok = ok && wait(aux.p_full[0], 0);
+        if (ok) scores(1, 0);
+      }
+    }
+    for (int j = 0; j < n_tiles && ok; ++j) {
+      const bool more = j + 1 < n_tiles;
+      ok = (!more || wait(aux.k_full, j + 1)) && wait(aux.v_full, j);
+      // S of the next key tile before the products that have to wait for this one's weights; its buffer held those of tile j - 1
+#pragma unroll
+      for (int t = 0; t < kTiles && ok; ++t) {
+        const bool some = t == 0 || second;
+        if (more) {
+          ok = j == 0 || wait(aux.o_done[t], j - 1);
+          if (!ok) break;
+          tc_fence_after();
+          scores(t, j + 1);
+        }
+        if (some) ok = wait(aux.p_full[t], j);
+        if (!ok) break;
+        tc_fence_after();
+        values(t, j);
+      }
     }
   } else {
     // ---- softmax: a thread per row; the warp's quarter of tensor memory is its number modulo 4 ----
@@ -334,8 +367,13 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_mag
     for (int j = 0; j < n_tiles && live; ++j) {
       const uint32_t s_at = lanes + (j & 1) * kKeys;
       const int seen = first + row - key0 - j * kKeys;   // the last token of the key tile that the row attends to
-      if (!wait(aux.s_full[tile], j) ||
-          !mbar_wait_warp(smem_u32(&aux.scales_full[j & 3]), (uint32_t)(j >> 2) & 1u, abort_flag, status, kStatusTileWait, lane)) {
+      const bool diagonal = key0 + j * kKeys + kKeys - 1 > first + tile * kRows;
+      const float2* scales = aux.scales[j & 3];
+      const uint32_t s_bar = smem_u32(&aux.s_full[tile][(j & 1)]), s_parity = (uint32_t)(j >> 1) & 1u;
+      const uint32_t f_bar = smem_u32(&aux.scales_full[j & 3]), f_parity = (uint32_t)(j >> 2) & 1u;
+      const bool there = mbar_try_wait_addr(f_bar, f_parity) & mbar_try_wait_addr(s_bar, s_parity);   // both round trips at once
+      if (!__all_sync(0xffffffffu, there) && !(mbar_wait_warp(f_bar, f_parity, abort_flag, status, kStatusTileWait, lane) &&
+                                               mbar_wait_warp(s_bar, s_parity, abort_flag, status, kStatusTileWait, lane))) {
         ok = false;
         break;
       }
@@ -343,18 +381,18 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_mag
       uint32_t v[kKeys];
       tmem_ld32(s_at, v);
       tmem_ld32(s_at + 32, v + 32);
-      float by[kGroups], lv[kGroups];
+      float by[kGroups], lv[kGroups], m_new = m, r_new = -INFINITY;
 #pragma unroll
       for (int b = 0; b < kGroups; ++b) {
-        const float2 s = aux.scales[j & 3][b];
-        by[b] = coef * s.x;
-        lv[b] = s.y;
+        by[b] = coef * scales[b].x;
+        lv[b] = scales[b].y;
       }
-      tmem_ld_wait();
-      if (key0 + j * kKeys + kKeys - 1 > first + tile * kRows) {   // the tile meets the diagonal
+      tmem_ld_wait32(v);
+      tmem_ld_wait32(v + 32);
+      if (diagonal) {
+        // -infinity times a factor that is 0 or NaN would be NaN: such a factor goes into the scores
 #pragma unroll
         for (int b = 0; b < kGroups; ++b) {
-          // -infinity times a factor that is 0 or NaN would be NaN: such a factor goes into the scores
           const bool plain = by[b] > 0.f;
           const uint32_t fill = by[b] == 0.f ? 0u : 0x7fc00000u;
           if (!plain) by[b] = 1.f;
@@ -362,12 +400,12 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_mag
           for (int i = 16 * b; i < 16 * b + 16; ++i) v[i] = i > seen ? 0xff800000u : plain ? v[i] : fill;
         }
       }
-      float m_new = m, r_new = -INFINITY;
 #pragma unroll
       for (int b = 0; b < kGroups; ++b) {
         float tops[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) tops[i / 2 & 1] = max3(tops[i / 2 & 1], __uint_as_float(v[16 * b + i]), __uint_as_float(v[16 * b + i + 1]));
+        for (int i = 16 * b; i < 16 * b + 16; i += 2)
+          tops[i / 2 & 1] = max3(tops[i / 2 & 1], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
         const float top = fmaxf(tops[0], tops[1]) * by[b];   // NaN counts as none
         m_new = fmaxf(m_new, top);
         r_new = fmaxf(r_new, top + lv[b]);
@@ -399,7 +437,7 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_mag
       // below -60 has no weight in fp16 either way
 #pragma unroll
       for (int b = 0; b < kGroups; ++b) {
-        const float off = base + lv[b] < -60.f ? -60.f : base + lv[b], from = off - shift;
+        const float at = base + lv[b], off = at < -60.f ? -60.f : at, from = off - shift;
         float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int i = 16 * b; i < 16 * b + 16; i += 2) {
@@ -411,15 +449,14 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_mag
         }
         sums[0] = add2(sums[0], sums[1]);
         l = fmaf(sums[0].x + sums[0].y, ex2(-off), l);
+        if (b & 1) tmem_st16(s_at + 8 * (b - 1), v + 8 * (b - 1));
       }
-      tmem_st16(s_at, v);
-      tmem_st16(s_at + 16, v + 16);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_addr(smem_u32(&aux.p_full[tile][j & 1]));
+      if (lane == 0) mbar_arrive_addr(smem_u32(&aux.p_full[tile][(j & 1)]));
     }
-    ok = ok && (n_tiles == 0 || wait(aux.v_empty, n_tiles - 1));
+    ok = ok && (n_tiles == 0 || !live || wait(aux.o_done[tile], n_tiles - 1));
     tc_fence_after();
     const float bad = __int_as_float(0x7fc00000);
     // O is relative to 2^(ref - kUp), the sum and the parts to 2^m
@@ -507,7 +544,7 @@ bool kv8_tiles_take(const Kv8Call& c) {
 
 // Parts that the tokens of a tile of rows are cut into: enough CTAs for two per SM, four key tiles each at least.
 int kv8_tile_splits(const Kv8Call& c) {
-  const int64_t tiles = ((int64_t)c.max_blocks * c.cache.block_size + kKeys - 1) / kKeys;
+  const int64_t tiles = ((int64_t)c.max_blocks * c.cache.block_size + 63) / 64;
   const int64_t units = (c.rows + kRows - 1) / kRows * c.cache.heads;   // at least
   int64_t n = ((int64_t)sm_count() * 2 + units - 1) / units;
   if (n > (tiles + 3) / 4) n = (tiles + 3) / 4;

@@ -80,12 +80,17 @@ def _write_fp8(dev, key, value, key_cache, value_cache, slot_mapping, k_scale, v
     for t in (key, value):
         if t.dim() != 3 or t.shape[1:] != (h, d) or t.stride(2) != 1 or (h > 1 and t.stride(1) != d):
             raise RuntimeError(f"reshape_and_cache_flash: key and value must be [T, {h}, {d}] with contiguous token rows")
-    slots = slot_mapping.contiguous()
+    slots = slot_mapping if slot_mapping.is_contiguous() else slot_mapping.contiguous()
+    n, lib = min(slots.numel(), key.shape[0], value.shape[0]), N.lib()
+    workspace, ws_bytes = None, lib.aps_kv8_write_workspace_bytes(n, nb)
+    if ws_bytes:
+        from .attention import _scratch_of
+        workspace, ws_bytes = _scratch_of(dev, ws_bytes)
     with N.on_device(dev):
-        N.check(N.lib().aps_kv8_write(
+        N.check(lib.aps_kv8_write(
             key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-            slots.data_ptr(), min(slots.numel(), key.shape[0], value.shape[0]), h, d, bs, nb, _row_stride(key), _row_stride(value),
-            key_cache.stride(0), k_scale.stride(0), N.dtype_enum(key), N.current_stream(dev)))
+            slots.data_ptr(), n, h, d, bs, nb, _row_stride(key), _row_stride(value), key_cache.stride(0), k_scale.stride(0),
+            N.ptr(workspace), ws_bytes, N.dtype_enum(key), N.current_stream(dev)))
 
 
 def prefill_cache_write(key: Optional[torch.Tensor], value: Optional[torch.Tensor],

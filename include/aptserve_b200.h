@@ -437,11 +437,14 @@ int aps_selftest_tile_pieces(int first, int last, int num_pieces, int* pieces_ou
  *    bytes and count as unwritten.
  *  - Otherwise the scale becomes the larger of the old one and the needed one; where it grows the block's other rows are rounded to it.
  * NaN and infinities are stored as NaN and have no part in the scale.
+ * workspace: aps_kv8_write_workspace_bytes(num_tokens, num_blocks) bytes, 256-byte aligned (NULL where that is 0, up to 1024 rows); its
+ * first 256 bytes, where the attention calls keep their status, are left alone.
  */
+size_t aps_kv8_write_workspace_bytes(int64_t num_tokens, int64_t num_blocks);
 int aps_kv8_write(const void* key, const void* value, void* key_cache, void* value_cache, float* key_scale, float* value_scale,
                   const int64_t* slot_mapping, int64_t num_tokens, int num_heads, int head_size, int block_size,
                   int64_t num_blocks, int64_t key_stride, int64_t value_stride, int64_t block_stride, int64_t scale_stride,
-                  int dtype, void* stream);
+                  void* workspace, size_t workspace_bytes, int dtype, void* stream);
 
 /*
  * Attention of query rows [num_rows, H, D] over that cache.  Row t belongs to the request r with query_start_loc[r] <= t <

@@ -20,7 +20,7 @@ def address(offset=0):
 
 def write(**kw):
     p = address()
-    a = dict(key=p, value=p, kc=p, vc=p, ks=p, vs=p, slots=p, t=2, h=2, d=64, bs=16, nb=4, s_k=128, s_v=128, block=2048, s_s=2, dtype=1)
+    a = dict(key=p, value=p, kc=p, vc=p, ks=p, vs=p, slots=p, t=2, h=2, d=64, bs=16, nb=4, s_k=128, s_v=128, block=2048, s_s=2, ws=p, ws_bytes=1 << 40, dtype=1)
     a.update(kw)
     return N.lib().aps_kv8_write(*a.values(), 0)
 
@@ -39,6 +39,7 @@ def attend(**kw):
     (N.APS_ERR_SHAPE, dict(s_k=64)), (N.APS_ERR_SHAPE, dict(block=1024)), (N.APS_ERR_SHAPE, dict(s_s=1)), (N.APS_ERR_SHAPE, dict(nb=1 << 28)),
     (N.APS_ERR_NULL_POINTER, dict(ks=0)), (N.APS_ERR_NULL_POINTER, dict(slots=0)), (N.APS_ERR_MISALIGNED, dict(kc=address(2))),
     (N.APS_ERR_MISALIGNED, dict(block=2050)), (N.APS_ERR_MISALIGNED, dict(key=address(1))), (N.APS_OK, dict(t=0, key=0)),
+    (N.APS_ERR_WORKSPACE, dict(t=1025, ws=0)), (N.APS_ERR_WORKSPACE, dict(t=1025, ws_bytes=1025 * 4)),
 ])
 def test_write_refuses(status, kw):
     assert write(**kw) == status
