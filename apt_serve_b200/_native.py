@@ -67,7 +67,7 @@ PROTOTYPES = {
                               [c_float, c_int, c_void_p]),
     "aps_kv8_write_workspace_bytes": (c_size_t, [c_int64, c_int64]),
     "aps_kv8_write": (c_int, [c_void_p] * 7 + [c_int64] + [c_int] * 3 + [c_int64] * 5 + [c_void_p, c_size_t, c_int, c_void_p]),
-    "aps_kv8_attention_workspace_bytes": (c_size_t, [c_int64] + [c_int] * 4),
+    "aps_kv8_attention_workspace_bytes": (c_size_t, [c_int, c_int64] + [c_int] * 4),
     "aps_kv8_attention": (c_int, [c_void_p] * 9 + [c_int, c_int64] + [c_int] * 5 + [c_int64] * 5 +
                           [c_float, c_void_p, c_size_t, c_int, c_void_p]),
     "aps_attention_status": (c_int, [c_void_p, c_void_p, c_void_p]),

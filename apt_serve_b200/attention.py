@@ -226,7 +226,7 @@ def _attend_fp8(op, query, key_cache, value_cache, block_tables, starts, seq_len
     lib = N.lib()
     with N.on_device(dev):
         if workspace is None:
-            workspace, ws_bytes = _scratch_of(dev, lib.aps_kv8_attention_workspace_bytes(t, bt.shape[1], bs, h, d))
+            workspace, ws_bytes = _scratch_of(dev, lib.aps_kv8_attention_workspace_bytes(b, t, bt.shape[1], bs, h, d))
         else:
             ws_bytes = workspace.numel() * workspace.element_size()
         N.check(lib.aps_kv8_attention(

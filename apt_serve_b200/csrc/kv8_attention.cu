@@ -2,6 +2,7 @@
 //
 //   kv8_rows_kernel     CUDA-core arithmetic, one CTA per (query row, head, part of the row's tokens): every query type, head size
 //                       and block stride.  D / 16 lanes cover a row with one 16-byte load each.
+//   (kv8_stream.cu)     up to 16 query rows per request, HBM-bound
 //   (kv8_prefix.cu)     several query rows per request on the tensor cores
 //   kv8_combine_kernel  joins the parts of rows whose tokens were cut.
 // Scores, softmax statistics and sums are fp32; a code times its scale is exact in fp32.
@@ -183,10 +184,14 @@ int launch_rows(const Kv8Call& c, const Kv8Parts& a, cudaStream_t stream) {
   return launch_status("kv8_rows_kernel");
 }
 
+enum Way { kRows, kStream, kTiles };
+
 template <typename T>
-int attend(const Kv8Call& c, const Kv8Parts& a, bool tiles, cudaStream_t stream) {
+int attend(const Kv8Call& c, const Kv8Parts& a, Way way, cudaStream_t stream) {
   int st;
-  if (tiles) {
+  if (way == kStream) {
+    st = launch_kv8_stream(c, a, stream);
+  } else if (way == kTiles) {
     st = launch_kv8_tiles(c, a, stream);
   } else {
     switch (c.cache.head_size) {
@@ -223,13 +228,17 @@ int check_call(const char* op, const Kv8Call& c) {
 
 using namespace aps;
 
-extern "C" size_t aps_kv8_attention_workspace_bytes(int64_t num_rows, int max_blocks_per_seq, int block_size, int num_heads, int head_size) {
-  if (num_rows <= 0 || max_blocks_per_seq <= 0 || block_size <= 0 || num_heads <= 0 || head_size <= 0) return 0;
+extern "C" size_t aps_kv8_attention_workspace_bytes(int batch, int64_t num_rows, int max_blocks_per_seq, int block_size, int num_heads, int head_size) {
+  if (batch <= 0 || num_rows <= 0 || max_blocks_per_seq <= 0 || block_size <= 0 || num_heads <= 0 || head_size <= 0) return 0;
   Kv8Call c{};
   c.rows = num_rows; c.max_blocks = max_blocks_per_seq;
   c.cache.heads = num_heads; c.cache.head_size = head_size; c.cache.block_size = block_size;
-  const int by_rows = row_splits(c), by_tiles = kv8_tile_splits(c);
-  return part_scratch(num_rows, num_heads, head_size, by_rows > by_tiles ? by_rows : by_tiles);
+  // the most that any of the kernels takes
+  c.batch = batch;
+  int most = row_splits(c);
+  if (kv8_stream_splits(c) > most) most = kv8_stream_splits(c);
+  if (kv8_tile_splits(c) > most) most = kv8_tile_splits(c);
+  return part_scratch(num_rows, num_heads, head_size, most);
 }
 
 extern "C" int aps_kv8_attention(void* out, const void* query, const void* key_cache, const void* value_cache, const float* key_scale,
@@ -247,8 +256,9 @@ extern "C" int aps_kv8_attention(void* out, const void* query, const void* key_c
   if (st != APS_OK || num_rows == 0 || batch == 0) return st;
   APS_REQUIRE(query_start_loc != nullptr || num_rows == batch, APS_ERR_SHAPE, "kv8_attention: %lld query rows for %d requests",
               (long long)num_rows, batch);
-  const bool tiles = kv8_tiles_take(c);
-  Kv8Parts a{static_cast<int*>(workspace), nullptr, nullptr, tiles ? kv8_tile_splits(c) : row_splits(c), scale * 1.4426950408889634f};
+  const Way way = kv8_stream_takes(c) ? kStream : kv8_tiles_take(c) ? kTiles : kRows;
+  Kv8Parts a{static_cast<int*>(workspace), nullptr, nullptr,
+             way == kStream ? kv8_stream_splits(c) : way == kTiles ? kv8_tile_splits(c) : row_splits(c), scale * 1.4426950408889634f};
   const size_t need = part_scratch(num_rows, num_heads, head_size, a.splits);
   APS_REQUIRE(workspace != nullptr && aligned_to(workspace, 256) && workspace_bytes >= need, APS_ERR_WORKSPACE,
               "kv8_attention: workspace must be 256-byte aligned and hold %zu bytes (got %zu)", need, workspace_bytes);
@@ -257,8 +267,8 @@ extern "C" int aps_kv8_attention(void* out, const void* query, const void* key_c
     a.acc = reinterpret_cast<float*>(static_cast<char*>(workspace) + part_acc_at(num_rows, num_heads, a.splits));
   }
   switch (dtype) {
-    case APS_F32: return attend<float>(c, a, tiles, (cudaStream_t)stream);
-    case APS_F16: return attend<__half>(c, a, tiles, (cudaStream_t)stream);
-    default: return attend<__nv_bfloat16>(c, a, tiles, (cudaStream_t)stream);
+    case APS_F32: return attend<float>(c, a, way, (cudaStream_t)stream);
+    case APS_F16: return attend<__half>(c, a, way, (cudaStream_t)stream);
+    default: return attend<__nv_bfloat16>(c, a, way, (cudaStream_t)stream);
   }
 }

@@ -93,6 +93,17 @@ __device__ __forceinline__ bool kv8_find_row(const Kv8Call& c, int64_t t, int& r
   return true;
 }
 
+// x / n by the high word of x * ceil(2^32 / n), n the blocks' size in groups of 16 tokens (up to 64): exact for x below 2^26.  0: n is 1.
+inline uint32_t kv8_blocks_magic(int block_size) {
+  const uint32_t n = block_size / 16;
+  return n == 1 ? 0u : (uint32_t)(((uint64_t(1) << 32) + n - 1) / n);
+}
+
+// Up to 16 query rows per request (kv8_stream.cu).
+bool kv8_stream_takes(const Kv8Call& c);
+int kv8_stream_splits(const Kv8Call& c);
+int launch_kv8_stream(const Kv8Call& c, const Kv8Parts& parts, cudaStream_t stream);
+
 // Query rows by tiles of 128 on the tensor cores (kv8_prefix.cu).
 bool kv8_tiles_take(const Kv8Call& c);
 int kv8_tile_splits(const Kv8Call& c);

@@ -521,9 +521,7 @@ int launch(const Kv8Call& c, const Kv8Parts& parts, cudaStream_t stream) {
   }
   const int vec = aligned_to(c.query, 16) && aligned_to(c.out, 16) && c.query_stride % 8 == 0 && c.out_stride % 8 == 0;
   const int blocks = (c.max_rows + kTiles * kRows - 1) / (kTiles * kRows);
-  // x / n = high word of x * ceil(2^32 / n), exact for x below 2^26 and n up to 64
-  const uint32_t n = c.cache.block_size / 16, magic = n == 1 ? 0u : (uint32_t)(((uint64_t(1) << 32) + n - 1) / n);
-  kernel<<<dim3(blocks * parts.splits, c.cache.heads, c.batch), (kSoftWarp + 4 * kTiles) * 32, smem, stream>>>(c, parts, magic, vec);
+  kernel<<<dim3(blocks * parts.splits, c.cache.heads, c.batch), (kSoftWarp + 4 * kTiles) * 32, smem, stream>>>(c, parts, kv8_blocks_magic(c.cache.block_size), vec);
   return launch_status("kv8_tile_kernel");
 }
 

@@ -452,9 +452,9 @@ int aps_kv8_write(const void* key, const void* value, void* key_cache, void* val
  * seq_lens[r] tokens, each attends to the tokens up to itself.  A row that attends to none (a length of 0, more rows than tokens) is
  * zero; rows before the first start and behind the last are left as they are.  max_query_len: no request has more rows.  A table entry
  * outside [0, num_blocks) is not read: the rows that attend to a token of it become NaN.
- * workspace: aps_kv8_attention_workspace_bytes(num_rows, ...) bytes, 256-byte aligned; aps_attention_status reads its status word.
+ * workspace: aps_kv8_attention_workspace_bytes(batch, num_rows, ...) bytes, 256-byte aligned; aps_attention_status reads its status word.
  */
-size_t aps_kv8_attention_workspace_bytes(int64_t num_rows, int max_blocks_per_seq, int block_size, int num_heads, int head_size);
+size_t aps_kv8_attention_workspace_bytes(int batch, int64_t num_rows, int max_blocks_per_seq, int block_size, int num_heads, int head_size);
 int aps_kv8_attention(void* out, const void* query, const void* key_cache, const void* value_cache, const float* key_scale,
                       const float* value_scale, const int32_t* block_tables, const int32_t* query_start_loc,
                       const int32_t* seq_lens, int batch, int64_t num_rows, int max_query_len, int max_blocks_per_seq,
