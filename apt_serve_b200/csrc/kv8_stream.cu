@@ -1,9 +1,9 @@
 // Up to 16 query rows per request over the 8-bit cache (kv8_common.cuh): decode, drafted tokens.  fp16 / bf16 queries, head sizes 64, 128.
 //
 // HBM-bound: the codes are read once, 2 D bytes a token and head.  One CTA of four warps per (request, head, part of the tokens); a warp
-// takes every fourth group of 16 tokens (which never straddles a block), its next groups already on their way to registers.  No shared
-// memory in between: the fragments of mma.sync.m16n8k16 are what 16-byte loads of the cache's rows give, if the dimensions are counted
-// in another order (a sum over them does not mind, and the output's columns are written where they belong):
+// takes every fourth group of 16 tokens (which never straddles a block), asynchronous copies bring its next groups to shared memory.
+// The fragments of mma.sync.m16n8k16 are what plain vector loads of the rows give there, if the dimensions are counted in another order
+// (a sum over them does not mind, and the output's columns are written where they belong):
 //   S = Q K^T   B (16 dims x 8 tokens): lane (g, j) = (lane / 4, lane % 4) holds four codes of token g at a time, of its 16 consecutive
 //               dims 16 j ... 16 j + 15 of a 64-byte half row; A holds the query's elements in the same order
 //   O += P V    B (16 tokens x 8 dims): the lane holds tokens 2 j, 2 j + 1, 2 j + 8, 2 j + 9 of its D / 8 consecutive dims; a byte
@@ -25,13 +25,37 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Loads that stay ahead of what is computed between them and their use.
-__device__ __forceinline__ void ld_ahead(const uint8_t* p, uint4& v) {
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+// 16 (or 4) bytes to shared memory; of which none: zeros.
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool some) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(some ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void ld_ahead(const uint8_t* p, uint2& v) {
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+__device__ __forceinline__ void copy4(uint32_t to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
 }
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
+__device__ __forceinline__ uint4 shared16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ uint2 shared8(uint32_t at) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ float2 shared_pair(uint32_t at) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at));
+  return v;
+}
+// Where piece c (16 bytes) of a row of D bytes lies in a group's 16 rows: 8 lanes' loads, of two tokens' pieces (K) or of four tokens'
+// (V), meet different banks (V at D = 64: two lanes each).
+template <int D> __device__ __forceinline__ uint32_t piece_at(int row, int c) {
+  if constexpr (D == 128) return (uint32_t)(row * 128 + ((c ^ (row & 7) ^ ((row & 1) << 2)) << 4));
+  else return (uint32_t)(row * 64 + ((c ^ (row >> 1 & 3)) << 4));
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -42,15 +66,15 @@ __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+template <int D> __host__ __device__ constexpr int stages() { return D == 128 ? 4 : 6; }   // groups of a warp in shared memory
+template <int D> __host__ __device__ constexpr int stage_bytes() { return 2 * 16 * D + 16; }
+
 // kHalves: of the 16 rows of a fragment, 1: up to 8 query rows, 2: up to 16.
 template <typename T, int D, int kHalves>
 __global__ void __launch_bounds__(kWarps * 32, kHalves == 1 ? 3 : 2)
 kv8_stream_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_magic, const int vec) {
-  constexpr int kCols = D / 64, kPer = D / 8;          // 64-byte pieces of a row; dims of a lane in V
-  constexpr int kAhead = D == 128 ? 2 : 4;             // groups of a warp in flight
-  using V = typename std::conditional<D == 128, uint4, uint2>::type;
-  struct Group { uint4 k[2][kCols]; V v[4]; float key_scale, value_scale; };
-  __shared__ float s_o[kWarps][8 * kHalves][D];
+  constexpr int kCols = D / 64, kPer = D / 8, kStages = stages<D>();   // 64-byte pieces of a row; dims of a lane in V
+  extern __shared__ __align__(128) uint8_t ring_raw[];                 // the warps' stages; in the end their outputs
   __shared__ float2 s_ml[kWarps][8 * kHalves];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
   const int head = blockIdx.x % c.cache.heads, part = blockIdx.x / c.cache.heads, req = part / parts.splits, split = part % parts.splits;
@@ -62,34 +86,39 @@ kv8_stream_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_m
   const int first = ctx - rows_all;                    // own position of the first row
   const int all = (ctx + 15) / 16, per = (all + parts.splits - 1) / parts.splits;   // groups of 16 tokens
   const int group0 = min(all, split * per), n_groups = min(all, group0 + per) - group0;
+  const int mine_groups = (n_groups - warp + kWarps - 1) / kWarps;                  // the warp's: warp, warp + 4, ...
   const int32_t* table = c.tables + (int64_t)req * c.max_blocks;
   const int64_t row_bytes = (int64_t)c.cache.heads * D;
-  const uint32_t per_block = (uint32_t)bs / 16;
+  const uint32_t per_block = (uint32_t)bs / 16, ring = (uint32_t)__cvta_generic_to_shared(ring_raw) + warp * (kStages * stage_bytes<D>());
   auto block_at = [&](uint32_t group) { return blocks_magic ? __umulhi(group, blocks_magic) : group; };   // group / per_block
-  auto block_of = [&](int i) { return i < n_groups ? table[block_at(group0 + i)] : -1; };
-  auto load = [&](Group& f, int i, int block) {
-    const uint32_t group = group0 + i;
+  auto block_of = [&](int k) { return k < mine_groups ? table[block_at(group0 + warp + k * kWarps)] : -1; };
+  // the warp's group k on its way to stage k % kStages
+  constexpr int kPieces = D / 16, kAtOnce = 32 / kPieces;
+  auto fetch = [&](int k, int block) {
+    const uint32_t group = group0 + warp + k * kWarps, to = ring + k % kStages * stage_bytes<D>();
     const bool in = block >= 0 && block < c.cache.num_blocks;
     if (!in) block = 0;   // something that can be read
-    const int64_t from = block * c.cache.block_stride + (int64_t)((group - block_at(group) * per_block) * 16) * row_bytes + (int64_t)head * D;
-    const uint8_t *k = c.cache.key + from + g * row_bytes + j * 16, *v = c.cache.value + from + 2 * j * row_bytes + g * kPer;
+    const int piece = lane % kPieces, r0 = lane / kPieces, live = in ? ctx - (int)group * 16 : 0;   // tokens that count
+    const int64_t from = block * c.cache.block_stride + (int64_t)((group - block_at(group) * per_block) * 16 + r0) * row_bytes +
+                         (int64_t)head * D + piece * 16;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int i = 0; i < 16 / kAtOnce; ++i) copy16(to + piece_at<D>(r0 + i * kAtOnce, piece), c.cache.key + from + i * kAtOnce * row_bytes, r0 + i * kAtOnce < live);
 #pragma unroll
-      for (int h = 0; h < kCols; ++h) ld_ahead(k + 8 * t * row_bytes + 64 * h, f.k[t][h]);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) ld_ahead(v + ((t & 1) + 8 * (t >> 1)) * row_bytes, f.v[t]);
-    const int64_t at = block * c.cache.scale_stride + head;
-    // a block outside the cache: the scores of its tokens are NaN
-    f.key_scale = in ? c.cache.key_scale[at] : __int_as_float(0x7fc00000);
-    f.value_scale = in ? c.cache.value_scale[at] : 0.f;
+    for (int i = 0; i < 16 / kAtOnce; ++i)
+      copy16(to + 16 * D + piece_at<D>(r0 + i * kAtOnce, piece), c.cache.value + from + i * kAtOnce * row_bytes, r0 + i * kAtOnce < live);
+    if (lane < 2) {
+      const uint32_t at = to + 2 * 16 * D + 4 * lane;
+      const int64_t place = block * c.cache.scale_stride + head;
+      if (in) copy4(at, (lane == 0 ? c.cache.key_scale : c.cache.value_scale) + place);
+      else asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(lane == 0 ? __int_as_float(0x7fc00000) : 0.f) : "memory");   // NaN scores
+    }
   };
-  Group buf[kAhead];
-  int next = block_of(warp);
+  int next = block_of(0);
 #pragma unroll
-  for (int u = 0; u < kAhead; ++u) {
-    if (warp + u * kWarps < n_groups) load(buf[u], warp + u * kWarps, next);
-    next = block_of(warp + (u + 1) * kWarps);
+  for (int k = 0; k < kStages - 1; ++k) {
+    if (k < mine_groups) fetch(k, next);
+    copy_commit();
+    next = block_of(k + 1);
   }
 
   // the query's fragments, rows g and g + 8: a half row's 16 dims of the lane, four at a time; bf16 as fp16 times a power of two per row
@@ -138,15 +167,18 @@ kv8_stream_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_m
 #pragma unroll
   for (int r = 0; r < kHalves; ++r) { m[r] = ref[r] = -INFINITY; l[r] = 0.f; }
 
-  auto consume = [&](Group& f, int i) {
-    const int t0 = (group0 + i) * 16;
+  auto consume = [&](int k) {
+    const int t0 = (group0 + warp + k * kWarps) * 16;
+    const uint32_t at = ring + k % kStages * stage_bytes<D>();
+    const float2 scales = shared_pair(at + 2 * 16 * D);
     float s[2][4];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
 #pragma unroll
       for (int h = 0; h < kCols; ++h) {
-        const uint32_t w[4] = {f.k[t][h].x, f.k[t][h].y, f.k[t][h].z, f.k[t][h].w};
+        const uint4 k4 = shared16(at + piece_at<D>(8 * t + g, 4 * h + j));
+        const uint32_t w[4] = {k4.x, k4.y, k4.z, k4.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint32_t* a = qa[4 * h + e];
@@ -155,14 +187,14 @@ kv8_stream_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_m
         }
       }
     }
-    const float lv = log2f(f.value_scale);
+    const float lv = log2f(scales.y);
     uint32_t p[2][2];   // [tokens' half][rows' half]
     const bool edge = t0 + 15 > first;   // some row does not attend to all of the tokens
     bool any = false;
     float down[kHalves];
 #pragma unroll
     for (int r = 0; r < kHalves; ++r) {
-      float by = coef[r] * f.key_scale;
+      float by = coef[r] * scales.x;
       if (edge) {
         // -infinity times a factor that is 0 or NaN would be NaN: such a factor goes into the scores
         const int seen = first + g + 8 * r - t0;   // the last token that the row attends to
@@ -206,14 +238,18 @@ kv8_stream_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_m
 #pragma unroll
         for (int r = 0; r < kHalves; ++r) { acc[n][2 * r] *= down[r]; acc[n][2 * r + 1] *= down[r]; }
     }
-    if (t0 + 16 > ctx) {   // rows behind the last token have no weight, but zero times whatever they hold might be NaN
+    uint32_t v[4][kPer / 4];   // tokens 2 j, 2 j + 1, 2 j + 8, 2 j + 9
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-        if (t0 + 2 * j + (t & 1) + 8 * (t >> 1) >= ctx) f.v[t] = V{};
+    for (int t = 0; t < 4; ++t) {
+      const int row = 2 * j + (t & 1) + 8 * (t >> 1);
+      if constexpr (D == 128) {
+        const uint4 x = shared16(at + 16 * D + piece_at<D>(row, g));
+        v[t][0] = x.x; v[t][1] = x.y; v[t][2] = x.z; v[t][3] = x.w;
+      } else {
+        const uint2 x = shared8(at + 16 * D + piece_at<D>(row, g >> 1) + 8 * (g & 1));
+        v[t][0] = x.x; v[t][1] = x.y;
+      }
     }
-    const uint32_t* v[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) v[t] = reinterpret_cast<const uint32_t*>(&f.v[t]);
 #pragma unroll
     for (int w = 0; w < kPer / 4; ++w) {
 #pragma unroll
@@ -226,17 +262,17 @@ kv8_stream_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_m
       }
     }
   };
-  for (int i = warp; i < n_groups; i += kAhead * kWarps) {
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int at = i + u * kWarps;
-      if (at < n_groups) {
-        consume(buf[u], at);
-        if (at + kAhead * kWarps < n_groups) load(buf[u], at + kAhead * kWarps, next);
-        next = block_of(at + (kAhead + 1) * kWarps);
-      }
-    }
+  for (int k = 0; k < mine_groups; ++k) {
+    copy_wait<kStages - 2>();
+    __syncwarp();   // every lane's copies of group k are there, every lane has read group k - 1
+    if (k + kStages - 1 < mine_groups) fetch(k + kStages - 1, next);
+    copy_commit();
+    next = block_of(k + kStages);
+    consume(k);
   }
+  copy_wait<0>();
+  __syncthreads();
+  float (*s_o)[8 * kHalves][D] = reinterpret_cast<float (*)[8 * kHalves][D]>(ring_raw);
 
   // the warps' shares, relative to 2^m
 #pragma unroll
@@ -280,10 +316,22 @@ kv8_stream_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_m
 
 template <typename T, int D, int kHalves>
 int launch(const Kv8Call& c, const Kv8Parts& parts, cudaStream_t stream) {
+  static bool done[64] = {false};
+  auto kernel = kv8_stream_kernel<T, D, kHalves>;
+  constexpr int smem = kWarps * stages<D>() * stage_bytes<D>();
+  static_assert(smem >= (int)sizeof(float) * kWarps * 8 * kHalves * D, "the outputs fit into the stages");
+  int dev = 0;
+  APS_CUDA(cudaGetDevice(&dev));
+  APS_REQUIRE(dev >= 0 && dev < 64, APS_ERR_CUDA, "device index %d out of range", dev);
+  if (!done[dev]) {
+    APS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    APS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+    done[dev] = true;
+  }
   const int64_t grid = (int64_t)c.batch * parts.splits * c.cache.heads;
   APS_REQUIRE(grid < (int64_t(1) << 31), APS_ERR_SHAPE, "kv8_attention: too many requests");
-  kv8_stream_kernel<T, D, kHalves><<<(unsigned)grid, kWarps * 32, 0, stream>>>(c, parts, kv8_blocks_magic(c.cache.block_size),
-                                                                                   aligned_to(c.query, 16) && c.query_stride % 8 == 0);
+  kernel<<<(unsigned)grid, kWarps * 32, smem, stream>>>(c, parts, kv8_blocks_magic(c.cache.block_size),
+                                                        aligned_to(c.query, 16) && c.query_stride % 8 == 0);
   return launch_status("kv8_stream_kernel");
 }
 
