@@ -123,18 +123,20 @@ kv8_rows_kernel(const Kv8Call c, const Kv8Parts a) {
   if (a.splits > 1 && threadIdx.x == 0) a.ml[unit] = make_float2(top, sum);
 }
 
-// One warp per (query row, head).
-template <typename T>
-__global__ void __launch_bounds__(256)
+// One warp per (query row, head): maximum and sum over the parts by lanes, then four elements of the output per lane (of a row of 32 or 64
+// the lanes share the parts), eight parts' loads at a time.  Always in the same order.
+template <typename T, int D>
+__global__ void __launch_bounds__(128)
 kv8_combine_kernel(const Kv8Call c, const Kv8Parts a) {
-  const int lane = threadIdx.x & 31, d = c.cache.head_size;
-  const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  constexpr int kLanes = D / 4 < 32 ? D / 4 : 32, kShare = 32 / kLanes, kPieces = D / (4 * kLanes);
+  const int lane = threadIdx.x & 31, share = lane / kLanes;
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (unit >= c.rows * c.cache.heads) return;
   const int64_t t = unit / c.cache.heads, h = unit % c.cache.heads;
   int req, keys;
-  if (!kv8_find_row(c, t, req, keys)) return;
+  const bool some = kv8_find_row(c, t, req, keys);
   const float2* ml = a.ml + unit * a.splits;
-  const float* acc = a.acc + unit * a.splits * d;
+  const float* acc = a.acc + unit * a.splits * D + lane % kLanes * 4;
   float top = -INFINITY, sum = 0.f;
   for (int i = lane; i < a.splits; i += 32) top = fmaxf(top, ml[i].x);
 #pragma unroll
@@ -143,12 +145,28 @@ kv8_combine_kernel(const Kv8Call c, const Kv8Parts a) {
   for (int i = lane; i < a.splits; i += 32) sum = fmaf(exp2f(ml[i].x - ref), ml[i].y, sum);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
-  T* out = static_cast<T*>(c.out) + t * c.out_stride + h * d;
-  for (int e = lane; e < d; e += 32) {
-    float x = 0.f;
-    for (int i = 0; i < a.splits; ++i)
-      if (ml[i].x != -INFINITY) x = fmaf(exp2f(ml[i].x - ref), acc[(int64_t)i * d + e], x);   // a part without tokens has no acc
-    out[e] = Elem<T>::from_float(keys == 0 ? 0.f : x / sum);
+  T* out = static_cast<T*>(c.out) + t * c.out_stride + h * D + lane % kLanes * 4;
+#pragma unroll
+  for (int p = 0; p < kPieces; ++p) {
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int i = share; i < a.splits; i += kShare) {
+      const float from = ml[i].x;
+      if (from == -INFINITY) continue;   // a part without tokens has no acc
+      const float w = exp2f(from - ref);
+      const float4 y = *reinterpret_cast<const float4*>(acc + (int64_t)i * D + 128 * p);
+      x.x = fmaf(w, y.x, x.x); x.y = fmaf(w, y.y, x.y); x.z = fmaf(w, y.z, x.z); x.w = fmaf(w, y.w, x.w);
+    }
+#pragma unroll
+    for (int o = kLanes; o < 32; o <<= 1) {
+      x.x += __shfl_xor_sync(kFull, x.x, o); x.y += __shfl_xor_sync(kFull, x.y, o);
+      x.z += __shfl_xor_sync(kFull, x.z, o); x.w += __shfl_xor_sync(kFull, x.w, o);
+    }
+    if (some && share == 0) {
+      const float y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[128 * p + e] = Elem<T>::from_float(keys == 0 ? 0.f : y[e] / sum);
+    }
   }
 }
 
@@ -172,7 +190,13 @@ size_t part_scratch(int64_t rows, int heads, int head_size, int splits) {
 template <typename T>
 int launch_parts_combine(const Kv8Call& c, const Kv8Parts& a, cudaStream_t stream) {
   if (a.splits == 1) return APS_OK;
-  kv8_combine_kernel<T><<<(unsigned)((c.rows * c.cache.heads + 7) / 8), 256, 0, stream>>>(c, a);
+  const unsigned grid = (unsigned)((c.rows * c.cache.heads + 3) / 4);
+  switch (c.cache.head_size) {
+    case 32: kv8_combine_kernel<T, 32><<<grid, 128, 0, stream>>>(c, a); break;
+    case 64: kv8_combine_kernel<T, 64><<<grid, 128, 0, stream>>>(c, a); break;
+    case 128: kv8_combine_kernel<T, 128><<<grid, 128, 0, stream>>>(c, a); break;
+    default: kv8_combine_kernel<T, 256><<<grid, 128, 0, stream>>>(c, a); break;
+  }
   return launch_status("kv8_combine_kernel");
 }
 

@@ -1,13 +1,16 @@
 // Up to 16 query rows per request over the 8-bit cache (kv8_common.cuh): decode, drafted tokens.  fp16 / bf16 queries, head sizes 64, 128.
 //
-// HBM-bound: the codes are read once, 2 D bytes a token and head.  One CTA of four warps per (request, head, part of the tokens); a warp
-// takes every fourth group of 16 tokens (which never straddles a block), asynchronous copies bring its next groups to shared memory.
-// The fragments of mma.sync.m16n8k16 are what plain vector loads of the rows give there, if the dimensions are counted in another order
-// (a sum over them does not mind, and the output's columns are written where they belong):
-//   S = Q K^T   B (16 dims x 8 tokens): lane (g, j) = (lane / 4, lane % 4) holds four codes of token g at a time, of its 16 consecutive
-//               dims 16 j ... 16 j + 15 of a 64-byte half row; A holds the query's elements in the same order
-//   O += P V    B (16 tokens x 8 dims): the lane holds tokens 2 j, 2 j + 1, 2 j + 8, 2 j + 9 of its D / 8 consecutive dims; a byte
-//               permutation pairs the tokens, and tile i of the output has dim (D / 8) n + i in column n
+// HBM-bound: the codes are read once, 2 D bytes a token and head.  One CTA of a single warp per (request, part of the tokens, head), the
+// heads next to one another, so that a token's row is read by warps that run at the same time; a group of 16 tokens (which never
+// straddles a block) at a time, asynchronous copies bring the next ones to shared memory.
+// Both products are taken the other way round, the cache's rows as the 16-row operand A of mma.sync.m16n8k16 and the query rows as the
+// 8 columns of B.  A's fragments are what plain vector loads of the rows give, if the dimensions are counted in another order (a sum over
+// them does not mind, and the output's are written where they belong); lane (g, j) = (lane / 4, lane % 4):
+//   S^T = K Q^T   A (16 tokens x 16 dims): four codes of token g and of token g + 8 at a time, of the lane's 16 consecutive dims
+//                 16 j ... 16 j + 15 of a 64-byte half row; B holds the query's elements in the same order
+//   O^T += V^T P^T  A (16 dims x 16 tokens): tokens 2 j, 2 j + 1, 2 j + 8, 2 j + 9 of the lane's D / 8 consecutive dims, the tokens
+//                 paired by a byte permutation; tile i has dims (D / 8) g + 2 i and + 1 in rows g and g + 8.  P^T comes from S^T's
+//                 layout by a transposition in registers (movmatrix)
 // Every e4m3 number is an fp16 number.  The scales and the weights' two references are those of the tile kernel (kv8_prefix.cu).
 #include "kv8_common.cuh"
 
@@ -17,7 +20,6 @@ namespace aps {
 namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
-constexpr int kWarps = 4;
 constexpr float kSlack = 8.f;   // log2 of how much the weights' reference may have grown before O is rescaled
 constexpr float kUp = 7.f;      // log2 of what the weights are kept at
 
@@ -25,7 +27,20 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {   // of an 8 x 8 matrix of 16-bit elements
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 // 16 (or 4) bytes to shared memory; of which none: zeros.
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
 __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool some) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(some ? 16 : 0) : "memory");
 }
@@ -66,67 +81,83 @@ __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// Groups of 16 tokens of a part, at least: 32, or as few as it takes for a warp of every place on the GPU (12 per SM), but 4.
+constexpr int64_t kUnits = 148 * 12;
+int part_groups(const Kv8Call& c) {
+  const int64_t groups = (int64_t)c.max_blocks * c.cache.block_size / 16 * c.batch * c.cache.heads;
+  const int64_t n = groups / kUnits;
+  return (int)(n < 4 ? 4 : n > 32 ? 32 : n);
+}
+
 template <int D> __host__ __device__ constexpr int stages() { return D == 128 ? 4 : 6; }   // groups of a warp in shared memory
 template <int D> __host__ __device__ constexpr int stage_bytes() { return 2 * 16 * D + 16; }
 
-// kHalves: of the 16 rows of a fragment, 1: up to 8 query rows, 2: up to 16.
-template <typename T, int D, int kHalves>
-__global__ void __launch_bounds__(kWarps * 32, kHalves == 1 ? 3 : 2)
-kv8_stream_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_magic, const int vec) {
+// kRows: query rows at most, 1, 8 or 16.
+template <typename T, int D, int kRows>
+__global__ void __launch_bounds__(32, kRows == 16 ? 10 : 12)
+kv8_stream_kernel(const Kv8Call c, const Kv8Parts parts, const int part_groups, const uint32_t blocks_magic, const int vec) {
   constexpr int kCols = D / 64, kPer = D / 8, kStages = stages<D>();   // 64-byte pieces of a row; dims of a lane in V
-  extern __shared__ __align__(128) uint8_t ring_raw[];                 // the warps' stages; in the end their outputs
-  __shared__ float2 s_ml[kWarps][8 * kHalves];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
+  constexpr int kSets = kRows == 16 ? 2 : 1, kEach = kRows == 1 ? 1 : 2;   // sets of 8 query rows; rows of a set whose softmax a lane keeps
+  extern __shared__ __align__(128) uint8_t ring_raw[];
+  const int lane = threadIdx.x, g = lane >> 2, j = lane & 3;
   const int head = blockIdx.x % c.cache.heads, part = blockIdx.x / c.cache.heads, req = part / parts.splits, split = part % parts.splits;
   if (blockIdx.x == 0 && threadIdx.x == 0) parts.plan[kPlanStatus] = kStatusOk;
   const int start = c.starts != nullptr ? c.starts[req] : req;
-  const int rows_all = c.starts != nullptr ? c.starts[req + 1] - start : 1, n_rows = min(8 * kHalves, rows_all);
+  const int rows_all = c.starts != nullptr ? c.starts[req + 1] - start : 1, n_rows = min(kRows, rows_all);
   if (n_rows <= 0) return;
   const int bs = c.cache.block_size, ctx = max(0, min(c.seq_lens[req], c.max_blocks * bs));
   const int first = ctx - rows_all;                    // own position of the first row
-  const int all = (ctx + 15) / 16, per = (all + parts.splits - 1) / parts.splits;   // groups of 16 tokens
+  const int all = (ctx + 15) / 16, per = max(part_groups, (all + parts.splits - 1) / parts.splits);   // groups of 16 tokens
   const int group0 = min(all, split * per), n_groups = min(all, group0 + per) - group0;
-  const int mine_groups = (n_groups - warp + kWarps - 1) / kWarps;                  // the warp's: warp, warp + 4, ...
   const int32_t* table = c.tables + (int64_t)req * c.max_blocks;
   const int64_t row_bytes = (int64_t)c.cache.heads * D;
-  const uint32_t per_block = (uint32_t)bs / 16, ring = (uint32_t)__cvta_generic_to_shared(ring_raw) + warp * (kStages * stage_bytes<D>());
+  const uint32_t per_block = (uint32_t)bs / 16, ring = (uint32_t)__cvta_generic_to_shared(ring_raw);
   auto block_at = [&](uint32_t group) { return blocks_magic ? __umulhi(group, blocks_magic) : group; };   // group / per_block
-  auto block_of = [&](int k) { return k < mine_groups ? table[block_at(group0 + warp + k * kWarps)] : -1; };
-  // the warp's group k on its way to stage k % kStages
-  constexpr int kPieces = D / 16, kAtOnce = 32 / kPieces;
+  auto block_of = [&](int k) { return k < n_groups ? table[block_at(group0 + k)] : -1; };
+  // group k on its way to stage k % kStages
+  constexpr int kPieces = D / 16, kAtOnce = 32 / kPieces, kCopies = 16 / kAtOnce;
+  const int piece = lane % kPieces, r0 = lane / kPieces;
+  const int64_t column = (int64_t)head * D + piece * 16 + r0 * row_bytes, step = kAtOnce * row_bytes;
+  const uint8_t *keys = c.cache.key + column, *values = c.cache.value + column;
+  const float* scales = (lane == 0 ? c.cache.key_scale : c.cache.value_scale) + head;
   auto fetch = [&](int k, int block) {
-    const uint32_t group = group0 + warp + k * kWarps, to = ring + k % kStages * stage_bytes<D>();
+    const uint32_t group = group0 + k, to = ring + k % kStages * stage_bytes<D>();
     const bool in = block >= 0 && block < c.cache.num_blocks;
     if (!in) block = 0;   // something that can be read
-    const int piece = lane % kPieces, r0 = lane / kPieces, live = in ? ctx - (int)group * 16 : 0;   // tokens that count
-    const int64_t from = block * c.cache.block_stride + (int64_t)((group - block_at(group) * per_block) * 16 + r0) * row_bytes +
-                         (int64_t)head * D + piece * 16;
+    const int64_t from = block * c.cache.block_stride + (int64_t)((group - block_at(group) * per_block) * 16) * row_bytes;
+    const uint8_t *kp = keys + from, *vp = values + from;
+    const int live = in ? ctx - (int)group * 16 : 0;   // tokens that count
+    if (live >= 16) {
 #pragma unroll
-    for (int i = 0; i < 16 / kAtOnce; ++i) copy16(to + piece_at<D>(r0 + i * kAtOnce, piece), c.cache.key + from + i * kAtOnce * row_bytes, r0 + i * kAtOnce < live);
+      for (int i = 0; i < kCopies; ++i) copy16(to + piece_at<D>(r0 + i * kAtOnce, piece), kp + i * step);
 #pragma unroll
-    for (int i = 0; i < 16 / kAtOnce; ++i)
-      copy16(to + 16 * D + piece_at<D>(r0 + i * kAtOnce, piece), c.cache.value + from + i * kAtOnce * row_bytes, r0 + i * kAtOnce < live);
+      for (int i = 0; i < kCopies; ++i) copy16(to + 16 * D + piece_at<D>(r0 + i * kAtOnce, piece), vp + i * step);
+    } else {              // rows behind the last token: zeros, whatever they hold
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) copy16(to + piece_at<D>(r0 + i * kAtOnce, piece), kp + i * step, r0 + i * kAtOnce < live);
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) copy16(to + 16 * D + piece_at<D>(r0 + i * kAtOnce, piece), vp + i * step, r0 + i * kAtOnce < live);
+    }
     if (lane < 2) {
       const uint32_t at = to + 2 * 16 * D + 4 * lane;
-      const int64_t place = block * c.cache.scale_stride + head;
-      if (in) copy4(at, (lane == 0 ? c.cache.key_scale : c.cache.value_scale) + place);
+      if (in) copy4(at, scales + block * c.cache.scale_stride);
       else asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(lane == 0 ? __int_as_float(0x7fc00000) : 0.f) : "memory");   // NaN scores
     }
   };
   int next = block_of(0);
 #pragma unroll
   for (int k = 0; k < kStages - 1; ++k) {
-    if (k < mine_groups) fetch(k, next);
+    if (k < n_groups) fetch(k, next);
     copy_commit();
     next = block_of(k + 1);
   }
 
-  // the query's fragments, rows g and g + 8: a half row's 16 dims of the lane, four at a time; bf16 as fp16 times a power of two per row
-  uint32_t qa[D / 16][2 * kHalves];
-  float coef[kHalves];
+  // the query's fragments, row g (and g + 8): a half row's 16 dims of the lane, four at a time; bf16 as fp16 times a power of two per row
+  uint32_t qb[kSets][D / 16][2];
+  float coef[kSets][kEach];
 #pragma unroll
-  for (int r = 0; r < kHalves; ++r) {
-    const int row = g + 8 * r;
+  for (int q = 0; q < kSets; ++q) {
+    const int row = g + 8 * q;
     const int64_t t = (int64_t)start + row;
     const bool mine = row < n_rows && t >= 0 && t < c.rows;
     const T* src = static_cast<const T*>(c.query) + (mine ? t : 0) * c.query_stride + (int64_t)head * D + j * 16;
@@ -152,91 +183,93 @@ kv8_stream_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_m
       down = __uint_as_float((uint32_t)(127 + p) << 23);
       up = __uint_as_float((uint32_t)(127 - p) << 23);
     }
-    coef[r] = parts.scale_log2 * up;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) coef[q][e] = parts.scale_log2 * __shfl_sync(kFull, up, kRows == 1 ? 0 : (2 * j + e) * 4);   // of row 2 j + e
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) {
-      qa[s][r] = half2_bits(x[4 * s] * down, x[4 * s + 1] * down);
-      qa[s][kHalves + r] = half2_bits(x[4 * s + 2] * down, x[4 * s + 3] * down);
+      qb[q][s][0] = half2_bits(x[4 * s] * down, x[4 * s + 1] * down);
+      qb[q][s][1] = half2_bits(x[4 * s + 2] * down, x[4 * s + 3] * down);
     }
   }
 
-  float acc[kPer][4];   // rows g, g, g + 8, g + 8
+  // columns 2 j, 2 j + 1 of a set are the lane's query rows
+  float acc[kSets][D / 16][4];   // dims' rows g, g, g + 8, g + 8
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-  float m[kHalves], l[kHalves], ref[kHalves];
+  for (int q = 0; q < kSets; ++q)
 #pragma unroll
-  for (int r = 0; r < kHalves; ++r) { m[r] = ref[r] = -INFINITY; l[r] = 0.f; }
+    for (int i = 0; i < D / 16; ++i) acc[q][i][0] = acc[q][i][1] = acc[q][i][2] = acc[q][i][3] = 0.f;
+  float m[kSets][kEach], l[kSets][kEach], ref[kSets][kEach];
+#pragma unroll
+  for (int q = 0; q < kSets; ++q)
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) { m[q][e] = ref[q][e] = -INFINITY; l[q][e] = 0.f; }
 
   auto consume = [&](int k) {
-    const int t0 = (group0 + warp + k * kWarps) * 16;
+    const int t0 = (group0 + k) * 16;
     const uint32_t at = ring + k % kStages * stage_bytes<D>();
-    const float2 scales = shared_pair(at + 2 * 16 * D);
-    float s[2][4];
+    const float2 scale = shared_pair(at + 2 * 16 * D);
+    float s[kSets][4];   // tokens g, g, g + 8, g + 8
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+    for (int q = 0; q < kSets; ++q) s[q][0] = s[q][1] = s[q][2] = s[q][3] = 0.f;
 #pragma unroll
-      for (int h = 0; h < kCols; ++h) {
-        const uint4 k4 = shared16(at + piece_at<D>(8 * t + g, 4 * h + j));
-        const uint32_t w[4] = {k4.x, k4.y, k4.z, k4.w};
+    for (int h = 0; h < kCols; ++h) {
+      const uint4 lo = shared16(at + piece_at<D>(g, 4 * h + j)), hi = shared16(at + piece_at<D>(g + 8, 4 * h + j));
+      const uint32_t w[2][4] = {{lo.x, lo.y, lo.z, lo.w}, {hi.x, hi.y, hi.z, hi.w}};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t* a = qa[4 * h + e];
-          mma16816(s[t], a[0], kHalves == 2 ? a[1] : 0u, a[kHalves], kHalves == 2 ? a[3] : 0u, e4m3x2_to_f16x2((uint16_t)w[e]),
-                   e4m3x2_to_f16x2((uint16_t)(w[e] >> 16)));
-        }
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t a0 = e4m3x2_to_f16x2((uint16_t)w[0][e]), a1 = e4m3x2_to_f16x2((uint16_t)w[1][e]);
+        const uint32_t a2 = e4m3x2_to_f16x2((uint16_t)(w[0][e] >> 16)), a3 = e4m3x2_to_f16x2((uint16_t)(w[1][e] >> 16));
+#pragma unroll
+        for (int q = 0; q < kSets; ++q) mma16816(s[q], a0, a1, a2, a3, qb[q][4 * h + e][0], qb[q][4 * h + e][1]);
       }
     }
-    const float lv = log2f(scales.y);
-    uint32_t p[2][2];   // [tokens' half][rows' half]
+    const float lv = lg2(scale.y);
+    uint32_t p[kSets][2];   // P^T's fragments
     const bool edge = t0 + 15 > first;   // some row does not attend to all of the tokens
     bool any = false;
-    float down[kHalves];
+    float down[kSets][2];
 #pragma unroll
-    for (int r = 0; r < kHalves; ++r) {
-      float by = coef[r] * scales.x;
-      if (edge) {
-        // -infinity times a factor that is 0 or NaN would be NaN: such a factor goes into the scores
-        const int seen = first + g + 8 * r - t0;   // the last token that the row attends to
-        const bool plain = by > 0.f;
-        const float fill = by == 0.f ? 0.f : __int_as_float(0x7fc00000);
-        if (!plain) by = 1.f;
+    for (int q = 0; q < kSets; ++q) {
+      float w[2][2] = {{0.f, 0.f}, {0.f, 0.f}};   // [tokens g, g + 8][rows]
+      down[q][1] = 1.f;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float& x = s[t][2 * r + e];
-            x = 8 * t + 2 * j + e > seen ? -INFINITY : plain ? x : fill;
-          }
-      }
-      float top = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
-      top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(kFull, top, 2)) * by;   // NaN counts as none
-      const float m_new = fmaxf(m[r], top), r_new = fmaxf(-INFINITY, top + lv);
-      const bool move = r_new > ref[r] && !(r_new - ref[r] <= kSlack);
-      any = any || move;
-      down[r] = move && ref[r] != -INFINITY ? ex2(ref[r] - r_new) : 1.f;
-      if (move) ref[r] = r_new;
-      const float shift = m_new == -INFINITY ? 0.f : m_new, base = shift - (ref[r] == -INFINITY ? 0.f : ref[r]) + kUp + lv;
-      const float off = base < -60.f ? -60.f : base, from = off - shift;
-      float x[4], sum = 0.f;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          x[2 * t + e] = ex2(fmaf(s[t][2 * r + e], by, from));
-          sum += x[2 * t + e];
+      for (int e = 0; e < kEach; ++e) {
+        float by = coef[q][e] * scale.x, x0 = s[q][e], x1 = s[q][2 + e];
+        if (edge) {
+          // -infinity times a factor that is 0 or NaN would be NaN: such a factor goes into the scores
+          const int seen = first + (kRows == 1 ? 0 : 8 * q + 2 * j + e) - t0;   // the last token that the row attends to
+          const bool plain = by > 0.f;
+          const float fill = by == 0.f ? 0.f : __int_as_float(0x7fc00000);
+          if (!plain) by = 1.f;
+          x0 = g > seen ? -INFINITY : plain ? x0 : fill;
+          x1 = g + 8 > seen ? -INFINITY : plain ? x1 : fill;
         }
-      l[r] = fmaf(sum, ex2(-off), m[r] == -INFINITY ? 0.f : l[r] * ex2(m[r] - shift));
-      m[r] = m_new;
-      p[0][r] = half2_bits(x[0], x[1]);
-      p[1][r] = half2_bits(x[2], x[3]);
+        float top = fmaxf(x0, x1);
+        top = fmaxf(top, __shfl_xor_sync(kFull, top, 4));
+        top = fmaxf(top, __shfl_xor_sync(kFull, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(kFull, top, 16)) * by;   // NaN counts as none
+        const float m_new = fmaxf(m[q][e], top), r_new = fmaxf(-INFINITY, top + lv);
+        const bool move = r_new > ref[q][e] && !(r_new - ref[q][e] <= kSlack);
+        any = any || move;
+        down[q][e] = move && ref[q][e] != -INFINITY ? ex2(ref[q][e] - r_new) : 1.f;
+        if (move) ref[q][e] = r_new;
+        const float shift = m_new == -INFINITY ? 0.f : m_new, base = shift - (ref[q][e] == -INFINITY ? 0.f : ref[q][e]) + kUp + lv;
+        const float off = base < -60.f ? -60.f : base, from = off - shift;
+        w[0][e] = ex2(fmaf(x0, by, from));
+        w[1][e] = ex2(fmaf(x1, by, from));
+        l[q][e] = fmaf(w[0][e] + w[1][e], ex2(-off), m[q][e] == -INFINITY ? 0.f : l[q][e] * ex2(m[q][e] - shift));
+        m[q][e] = m_new;
+      }
+      p[q][0] = transposed(half2_bits(w[0][0], w[0][1]));
+      p[q][1] = transposed(half2_bits(w[1][0], w[1][1]));
     }
     if (__any_sync(kFull, any)) {
 #pragma unroll
-      for (int n = 0; n < kPer; ++n)
+      for (int q = 0; q < kSets; ++q)
 #pragma unroll
-        for (int r = 0; r < kHalves; ++r) { acc[n][2 * r] *= down[r]; acc[n][2 * r + 1] *= down[r]; }
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[q][i][e] *= down[q][e & 1];
     }
     uint32_t v[4][kPer / 4];   // tokens 2 j, 2 j + 1, 2 j + 8, 2 j + 9
 #pragma unroll
@@ -251,75 +284,72 @@ kv8_stream_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_m
       }
     }
 #pragma unroll
-    for (int w = 0; w < kPer / 4; ++w) {
+    for (int i = 0; i < D / 16; ++i) {   // dims 2 i and 2 i + 1 of the lane's
+      const uint32_t b0 = __byte_perm(v[0][i / 2], v[1][i / 2], i & 1 ? 0x7362 : 0x5140);
+      const uint32_t b1 = __byte_perm(v[2][i / 2], v[3][i / 2], i & 1 ? 0x7362 : 0x5140);
+      const uint32_t a0 = e4m3x2_to_f16x2((uint16_t)b0), a1 = e4m3x2_to_f16x2((uint16_t)(b0 >> 16));
+      const uint32_t a2 = e4m3x2_to_f16x2((uint16_t)b1), a3 = e4m3x2_to_f16x2((uint16_t)(b1 >> 16));
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const uint32_t b0 = __byte_perm(v[0][w], v[1][w], e ? 0x7362 : 0x5140), b1 = __byte_perm(v[2][w], v[3][w], e ? 0x7362 : 0x5140);
-#pragma unroll
-        for (int o = 0; o < 2; ++o)
-          mma16816(acc[4 * w + 2 * e + o], p[0][0], kHalves == 2 ? p[0][1] : 0u, p[1][0], kHalves == 2 ? p[1][1] : 0u,
-                   e4m3x2_to_f16x2((uint16_t)(b0 >> 16 * o)), e4m3x2_to_f16x2((uint16_t)(b1 >> 16 * o)));
-      }
+      for (int q = 0; q < kSets; ++q) mma16816(acc[q][i], a0, a1, a2, a3, p[q][0], p[q][1]);
     }
   };
-  for (int k = 0; k < mine_groups; ++k) {
+  for (int k = 0; k < n_groups; ++k) {
     copy_wait<kStages - 2>();
     __syncwarp();   // every lane's copies of group k are there, every lane has read group k - 1
-    if (k + kStages - 1 < mine_groups) fetch(k + kStages - 1, next);
+    if (k + kStages - 1 < n_groups) fetch(k + kStages - 1, next);
     copy_commit();
     next = block_of(k + kStages);
     consume(k);
   }
   copy_wait<0>();
-  __syncthreads();
-  float (*s_o)[8 * kHalves][D] = reinterpret_cast<float (*)[8 * kHalves][D]>(ring_raw);
 
-  // the warps' shares, relative to 2^m
+  // the rows: the lane has dims kPer g ... kPer g + kPer - 1 of its query rows
 #pragma unroll
-  for (int r = 0; r < kHalves; ++r) {
-    const int row = g + 8 * r;
-    l[r] += __shfl_xor_sync(kFull, l[r], 1);
-    l[r] += __shfl_xor_sync(kFull, l[r], 2);
-    const float by = ref[r] == -INFINITY ? 0.f : ex2(ref[r] - kUp - (m[r] == -INFINITY ? 0.f : m[r]));
-    if (row < n_rows) {
+  for (int q = 0; q < kSets; ++q)
 #pragma unroll
-      for (int n = 0; n < kPer; ++n)
+    for (int e = 0; e < kEach; ++e) {
+      const int row = 8 * q + 2 * j + e;
+      const int64_t t = (int64_t)start + row;
+      float sum = l[q][e];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) s_o[warp][row][(2 * j + e) * kPer + n] = acc[n][2 * r + e] * by;
-      if (j == 0) s_ml[warp][row] = make_float2(m[r], l[r]);
+      for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(kFull, sum, o);
+      if (row >= n_rows || t < 0 || t >= c.rows) continue;
+      float by = ref[q][e] == -INFINITY ? 0.f : ex2(ref[q][e] - kUp - (m[q][e] == -INFINITY ? 0.f : m[q][e]));   // relative to 2^m
+      if (parts.splits == 1) by /= sum;    // nothing but scores of -infinity: NaN
+      const bool none = first + row < 0;   // a row before the first token
+      const int64_t unit = (t * c.cache.heads + head) * parts.splits + split;
+      float x[kPer];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) x[i] = none ? 0.f : acc[q][i / 2][2 * (i & 1) + e] * by;
+      if (parts.splits > 1) {
+        float* dst = parts.acc + unit * D + kPer * g;
+#pragma unroll
+        for (int i = 0; i < kPer; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+        if (g == 0) parts.ml[unit] = make_float2(m[q][e], sum);
+      } else {
+        T* dst = static_cast<T*>(c.out) + t * c.out_stride + (int64_t)head * D + kPer * g;
+        if (vec) {
+          struct alignas(16) Eight { T x[8]; };
+#pragma unroll
+          for (int i = 0; i < kPer; i += 8) {
+            Eight o;
+#pragma unroll
+            for (int d = 0; d < 8; ++d) o.x[d] = Elem<T>::from_float(x[i + d]);
+            *reinterpret_cast<Eight*>(dst + i) = o;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) dst[i] = Elem<T>::from_float(x[i]);
+        }
+      }
     }
-  }
-  __syncthreads();
-  for (int at = threadIdx.x; at < n_rows * D; at += kWarps * 32) {
-    const int row = at / D, d = at % D;
-    const int64_t t = (int64_t)start + row;
-    if (t < 0 || t >= c.rows) continue;
-    float top = -INFINITY, sum = 0.f, x = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_ml[w][row].x);
-    const float shift = top == -INFINITY ? 0.f : top;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float by = ex2(s_ml[w][row].x - shift);
-      sum = fmaf(by, s_ml[w][row].y, sum);
-      x = fmaf(by, s_o[w][row][d], x);
-    }
-    const int64_t unit = (t * c.cache.heads + head) * parts.splits + split;
-    if (parts.splits == 1) {
-      static_cast<T*>(c.out)[t * c.out_stride + (int64_t)head * D + d] = Elem<T>::from_float(first + row < 0 ? 0.f : x / sum);
-    } else {
-      parts.acc[unit * D + d] = x;
-      if (d == 0) parts.ml[unit] = make_float2(top, sum);
-    }
-  }
 }
 
-template <typename T, int D, int kHalves>
+template <typename T, int D, int kRows>
 int launch(const Kv8Call& c, const Kv8Parts& parts, cudaStream_t stream) {
   static bool done[64] = {false};
-  auto kernel = kv8_stream_kernel<T, D, kHalves>;
-  constexpr int smem = kWarps * stages<D>() * stage_bytes<D>();
-  static_assert(smem >= (int)sizeof(float) * kWarps * 8 * kHalves * D, "the outputs fit into the stages");
+  auto kernel = kv8_stream_kernel<T, D, kRows>;
+  constexpr int smem = stages<D>() * stage_bytes<D>();
   int dev = 0;
   APS_CUDA(cudaGetDevice(&dev));
   APS_REQUIRE(dev >= 0 && dev < 64, APS_ERR_CUDA, "device index %d out of range", dev);
@@ -330,16 +360,20 @@ int launch(const Kv8Call& c, const Kv8Parts& parts, cudaStream_t stream) {
   }
   const int64_t grid = (int64_t)c.batch * parts.splits * c.cache.heads;
   APS_REQUIRE(grid < (int64_t(1) << 31), APS_ERR_SHAPE, "kv8_attention: too many requests");
-  kernel<<<(unsigned)grid, kWarps * 32, smem, stream>>>(c, parts, kv8_blocks_magic(c.cache.block_size),
-                                                        aligned_to(c.query, 16) && c.query_stride % 8 == 0);
+  const int vec = aligned_to(c.query, 16) && aligned_to(c.out, 16) && c.query_stride % 8 == 0 && c.out_stride % 8 == 0;
+  kernel<<<(unsigned)grid, 32, smem, stream>>>(c, parts, part_groups(c), kv8_blocks_magic(c.cache.block_size), vec);
   return launch_status("kv8_stream_kernel");
+}
+
+template <typename T, int D>
+int launch_rows(const Kv8Call& c, const Kv8Parts& parts, cudaStream_t stream) {
+  if (c.starts == nullptr || c.max_rows == 1) return launch<T, D, 1>(c, parts, stream);
+  return c.max_rows <= 8 ? launch<T, D, 8>(c, parts, stream) : launch<T, D, 16>(c, parts, stream);
 }
 
 template <typename T>
 int launch_typed(const Kv8Call& c, const Kv8Parts& parts, cudaStream_t stream) {
-  const bool two = c.max_rows > 8;
-  if (c.cache.head_size == 128) return two ? launch<T, 128, 2>(c, parts, stream) : launch<T, 128, 1>(c, parts, stream);
-  return two ? launch<T, 64, 2>(c, parts, stream) : launch<T, 64, 1>(c, parts, stream);
+  return c.cache.head_size == 128 ? launch_rows<T, 128>(c, parts, stream) : launch_rows<T, 64>(c, parts, stream);
 }
 
 }  // namespace
@@ -349,12 +383,12 @@ bool kv8_stream_takes(const Kv8Call& c) {
          (c.cache.head_size == 64 || c.cache.head_size == 128) && c.cache.num_blocks > 0 && c.scale >= 1.17549435e-38f && c.scale < 1.70141183e38f;
 }
 
-// Parts that a request's tokens are cut into: enough CTAs for eight per SM, 256 tokens of the tables' width each at least.
+// Parts that a request's tokens are cut into.
 int kv8_stream_splits(const Kv8Call& c) {
-  const int64_t units = (int64_t)c.batch * c.cache.heads, tokens = (int64_t)c.max_blocks * c.cache.block_size;
-  const int64_t want = ((int64_t)sm_count() * 8 + units - 1) / units, most = (tokens + 255) / 256;
-  const int64_t n = want < most ? want : most;
-  return (int)(n < 1 ? 1 : n > 1024 ? 1024 : n);
+  const int64_t groups = (int64_t)c.max_blocks * c.cache.block_size / 16, n = (groups + part_groups(c) - 1) / part_groups(c);
+  // with many units and wide tables (of which the lengths may use little) no more than a few
+  const int64_t units = (int64_t)c.batch * c.cache.heads, most = (kUnits * 4 + units - 1) / units;
+  return (int)(n < most ? n : most < 4 ? (n < 4 ? n : 4) : most);
 }
 
 int launch_kv8_stream(const Kv8Call& c, const Kv8Parts& parts, cudaStream_t stream) {
