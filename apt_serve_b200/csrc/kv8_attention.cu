@@ -19,6 +19,8 @@ __global__ void __launch_bounds__(kRowWarps * 32)
 kv8_rows_kernel(const Kv8Call c, const Kv8Parts a) {
   constexpr int kLanes = D / 16, kTok = 32 / kLanes, kLoads = 4;   // lanes per row, rows per load, loads at a time
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % kLanes, tsel = lane / kLanes;
+  chain_wait();
+  chain_next();
   const int64_t t = blockIdx.x / a.splits;
   const int split = (int)(blockIdx.x % a.splits), h = blockIdx.y;
   if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) a.plan[kPlanStatus] = kStatusOk;
@@ -123,50 +125,63 @@ kv8_rows_kernel(const Kv8Call c, const Kv8Parts a) {
   if (a.splits > 1 && threadIdx.x == 0) a.ml[unit] = make_float2(top, sum);
 }
 
-// One warp per (query row, head): maximum and sum over the parts by lanes, then four elements of the output per lane (of a row of 32 or 64
-// the lanes share the parts), eight parts' loads at a time.  Always in the same order.
+// One CTA per (query row, head): the parts' weights first, then D / 4 lanes take four elements of the output each, the others share the
+// parts.  Always in the same order.  (A warp per row took 18 us over 118 parts of one row, one part after the other.)
+constexpr int kMostParts = 1024;
+
 template <typename T, int D>
 __global__ void __launch_bounds__(128)
 kv8_combine_kernel(const Kv8Call c, const Kv8Parts a) {
-  constexpr int kLanes = D / 4 < 32 ? D / 4 : 32, kShare = 32 / kLanes, kPieces = D / (4 * kLanes);
-  const int lane = threadIdx.x & 31, share = lane / kLanes;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (unit >= c.rows * c.cache.heads) return;
-  const int64_t t = unit / c.cache.heads, h = unit % c.cache.heads;
+  constexpr int kLanes = D / 4, kShare = 128 / kLanes;
+  __shared__ float s_w[kMostParts];
+  __shared__ float s_red[2][4];
+  __shared__ __align__(16) float4 s_x[128];
+  chain_wait();
+  chain_next();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, d = tid % kLanes * 4, share = tid / kLanes;
+  const int64_t unit = blockIdx.x, t = unit / c.cache.heads, h = unit % c.cache.heads;
   int req, keys;
-  const bool some = kv8_find_row(c, t, req, keys);
+  if (!kv8_find_row(c, t, req, keys)) return;
   const float2* ml = a.ml + unit * a.splits;
-  const float* acc = a.acc + unit * a.splits * D + lane % kLanes * 4;
+  const float* acc = a.acc + unit * a.splits * D + d;
   float top = -INFINITY, sum = 0.f;
-  for (int i = lane; i < a.splits; i += 32) top = fmaxf(top, ml[i].x);
+  for (int i = tid; i < a.splits; i += 128) top = fmaxf(top, ml[i].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+  if (lane == 0) s_red[0][warp] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
   const float ref = top == -INFINITY ? 0.f : top;
-  for (int i = lane; i < a.splits; i += 32) sum = fmaf(exp2f(ml[i].x - ref), ml[i].y, sum);
+  for (int i = tid; i < a.splits; i += 128) {
+    const float2 x = ml[i];
+    const float w = exp2f(x.x - ref);
+    sum = fmaf(w, x.y, sum);
+    s_w[i] = x.x == -INFINITY ? -1.f : w;   // a part without tokens has no acc
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
-  T* out = static_cast<T*>(c.out) + t * c.out_stride + h * D + lane % kLanes * 4;
+  if (lane == 0) s_red[1][warp] = sum;
+  __syncthreads();
+  sum = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = share; i < a.splits; i += kShare) {
+    const float w = s_w[i];
+    const float4 y = w < 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : *reinterpret_cast<const float4*>(acc + (int64_t)i * D);
+    x.x = fmaf(w, y.x, x.x); x.y = fmaf(w, y.y, x.y); x.z = fmaf(w, y.z, x.z); x.w = fmaf(w, y.w, x.w);
+  }
+  s_x[tid] = x;
+  __syncthreads();
+  if (share == 0) {
 #pragma unroll
-  for (int p = 0; p < kPieces; ++p) {
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int i = share; i < a.splits; i += kShare) {
-      const float from = ml[i].x;
-      if (from == -INFINITY) continue;   // a part without tokens has no acc
-      const float w = exp2f(from - ref);
-      const float4 y = *reinterpret_cast<const float4*>(acc + (int64_t)i * D + 128 * p);
-      x.x = fmaf(w, y.x, x.x); x.y = fmaf(w, y.y, x.y); x.z = fmaf(w, y.z, x.z); x.w = fmaf(w, y.w, x.w);
+    for (int i = 1; i < kShare; ++i) {
+      const float4 y = s_x[tid + i * kLanes];
+      x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
     }
+    const float y[4] = {x.x, x.y, x.z, x.w};
+    T* out = static_cast<T*>(c.out) + t * c.out_stride + h * D + d;
 #pragma unroll
-    for (int o = kLanes; o < 32; o <<= 1) {
-      x.x += __shfl_xor_sync(kFull, x.x, o); x.y += __shfl_xor_sync(kFull, x.y, o);
-      x.z += __shfl_xor_sync(kFull, x.z, o); x.w += __shfl_xor_sync(kFull, x.w, o);
-    }
-    if (some && share == 0) {
-      const float y[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) out[128 * p + e] = Elem<T>::from_float(keys == 0 ? 0.f : y[e] / sum);
-    }
+    for (int e = 0; e < 4; ++e) out[e] = Elem<T>::from_float(keys == 0 ? 0.f : y[e] / sum);
   }
 }
 
@@ -175,7 +190,7 @@ int row_splits(const Kv8Call& c) {
   const int64_t units = c.rows * c.cache.heads, tokens = (int64_t)c.max_blocks * c.cache.block_size;
   const int64_t want = ((int64_t)sm_count() * 8 + units - 1) / units, most = (tokens + 255) / 256;
   const int64_t n = want < most ? want : most;
-  return (int)(n < 1 ? 1 : n > 1024 ? 1024 : n);
+  return (int)(n < 1 ? 1 : n > kMostParts ? kMostParts : n);
 }
 
 // The scratch: header, maxima and sums, weighted values (16-byte stores).
@@ -190,22 +205,21 @@ size_t part_scratch(int64_t rows, int heads, int head_size, int splits) {
 template <typename T>
 int launch_parts_combine(const Kv8Call& c, const Kv8Parts& a, cudaStream_t stream) {
   if (a.splits == 1) return APS_OK;
-  const unsigned grid = (unsigned)((c.rows * c.cache.heads + 3) / 4);
+  const int64_t grid = c.rows * c.cache.heads;
+  APS_REQUIRE(grid < (int64_t(1) << 31), APS_ERR_SHAPE, "kv8_attention: too many rows");
   switch (c.cache.head_size) {
-    case 32: kv8_combine_kernel<T, 32><<<grid, 128, 0, stream>>>(c, a); break;
-    case 64: kv8_combine_kernel<T, 64><<<grid, 128, 0, stream>>>(c, a); break;
-    case 128: kv8_combine_kernel<T, 128><<<grid, 128, 0, stream>>>(c, a); break;
-    default: kv8_combine_kernel<T, 256><<<grid, 128, 0, stream>>>(c, a); break;
+    case 32: return launch_chained("kv8_combine_kernel", kv8_combine_kernel<T, 32>, (unsigned)grid, 128, 0, stream, c, a);
+    case 64: return launch_chained("kv8_combine_kernel", kv8_combine_kernel<T, 64>, (unsigned)grid, 128, 0, stream, c, a);
+    case 128: return launch_chained("kv8_combine_kernel", kv8_combine_kernel<T, 128>, (unsigned)grid, 128, 0, stream, c, a);
+    default: return launch_chained("kv8_combine_kernel", kv8_combine_kernel<T, 256>, (unsigned)grid, 128, 0, stream, c, a);
   }
-  return launch_status("kv8_combine_kernel");
 }
 
 template <typename T, int D>
 int launch_rows(const Kv8Call& c, const Kv8Parts& a, cudaStream_t stream) {
   const int64_t grid = c.rows * a.splits;
   APS_REQUIRE(grid < (int64_t(1) << 31), APS_ERR_SHAPE, "kv8_attention: too many rows");
-  kv8_rows_kernel<T, D><<<dim3((unsigned)grid, c.cache.heads), kRowWarps * 32, 0, stream>>>(c, a);
-  return launch_status("kv8_rows_kernel");
+  return launch_chained("kv8_rows_kernel", kv8_rows_kernel<T, D>, dim3((unsigned)grid, c.cache.heads), kRowWarps * 32, 0, stream, c, a);
 }
 
 enum Way { kRows, kStream, kTiles };

@@ -112,12 +112,13 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_mag
   extern __shared__ uint8_t smem_raw[];
   const uint32_t q_at = (smem_u32(smem_raw) + 1023) & ~1023u, k_at = q_at + kTiles * kQBytes, v_at = k_at + 2 * kTileBytes;
   __shared__ Aux<kTiles> aux;
+  chain_wait();
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int head = blockIdx.y, req = blockIdx.z, splits = parts.splits, split = blockIdx.x % splits;
   if (blockIdx.x == 0 && head == 0 && req == 0 && threadIdx.x == 0) parts.plan[kPlanStatus] = kStatusOk;
   const int start = c.starts[req], n_rows = c.starts[req + 1] - start;
   const int row0 = (int)(gridDim.x / splits - 1 - blockIdx.x / splits) * (kTiles * kRows);    // the rows with the most tokens first
-  if (row0 >= n_rows) return;
+  if (row0 >= n_rows) { chain_next(); return; }
   const int bs = c.cache.block_size, ctx = max(0, min(c.seq_lens[req], c.max_blocks * bs));
   const int first = ctx - n_rows + row0;                                 // own position of the CTA's first row
   const int rows_here = min(kTiles * kRows, n_rows - row0);
@@ -143,6 +144,7 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_mag
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  chain_next();
   const uint32_t tmem = aux.tmem_base;
   volatile int* abort_flag = &aux.abort_flag;
   int* status = parts.plan + kPlanStatus;
@@ -521,8 +523,8 @@ int launch(const Kv8Call& c, const Kv8Parts& parts, cudaStream_t stream) {
   }
   const int vec = aligned_to(c.query, 16) && aligned_to(c.out, 16) && c.query_stride % 8 == 0 && c.out_stride % 8 == 0;
   const int blocks = (c.max_rows + kTiles * kRows - 1) / (kTiles * kRows);
-  kernel<<<dim3(blocks * parts.splits, c.cache.heads, c.batch), (kSoftWarp + 4 * kTiles) * 32, smem, stream>>>(c, parts, kv8_blocks_magic(c.cache.block_size), vec);
-  return launch_status("kv8_tile_kernel");
+  return launch_chained("kv8_tile_kernel", kernel, dim3(blocks * parts.splits, c.cache.heads, c.batch), (kSoftWarp + 4 * kTiles) * 32, smem,
+                        stream, c, parts, kv8_blocks_magic(c.cache.block_size), vec);
 }
 
 template <typename T>

@@ -100,6 +100,8 @@ kv8_stream_kernel(const Kv8Call c, const Kv8Parts parts, const int part_groups, 
   constexpr int kSets = kRows == 16 ? 2 : 1, kEach = kRows == 1 ? 1 : 2;   // sets of 8 query rows; rows of a set whose softmax a lane keeps
   extern __shared__ __align__(128) uint8_t ring_raw[];
   const int lane = threadIdx.x, g = lane >> 2, j = lane & 3;
+  chain_wait();
+  chain_next();
   const int head = blockIdx.x % c.cache.heads, part = blockIdx.x / c.cache.heads, req = part / parts.splits, split = part % parts.splits;
   if (blockIdx.x == 0 && threadIdx.x == 0) parts.plan[kPlanStatus] = kStatusOk;
   const int start = c.starts != nullptr ? c.starts[req] : req;
@@ -361,8 +363,8 @@ int launch(const Kv8Call& c, const Kv8Parts& parts, cudaStream_t stream) {
   const int64_t grid = (int64_t)c.batch * parts.splits * c.cache.heads;
   APS_REQUIRE(grid < (int64_t(1) << 31), APS_ERR_SHAPE, "kv8_attention: too many requests");
   const int vec = aligned_to(c.query, 16) && aligned_to(c.out, 16) && c.query_stride % 8 == 0 && c.out_stride % 8 == 0;
-  kernel<<<(unsigned)grid, 32, smem, stream>>>(c, parts, part_groups(c), kv8_blocks_magic(c.cache.block_size), vec);
-  return launch_status("kv8_stream_kernel");
+  return launch_chained("kv8_stream_kernel", kernel, (unsigned)grid, 32, smem, stream, c, parts, part_groups(c),
+                        kv8_blocks_magic(c.cache.block_size), vec);
 }
 
 template <typename T, int D>
@@ -388,7 +390,8 @@ int kv8_stream_splits(const Kv8Call& c) {
   const int64_t groups = (int64_t)c.max_blocks * c.cache.block_size / 16, n = (groups + part_groups(c) - 1) / part_groups(c);
   // with many units and wide tables (of which the lengths may use little) no more than a few
   const int64_t units = (int64_t)c.batch * c.cache.heads, most = (kUnits * 4 + units - 1) / units;
-  return (int)(n < most ? n : most < 4 ? (n < 4 ? n : 4) : most);
+  const int64_t some = n < most ? n : most < 4 ? (n < 4 ? n : 4) : most;
+  return (int)(some > 1024 ? 1024 : some);   // as many as the joining kernel takes
 }
 
 int launch_kv8_stream(const Kv8Call& c, const Kv8Parts& parts, cudaStream_t stream) {

@@ -222,6 +222,8 @@ kv8_write_kernel(const WriteArgs a) {
   extern __shared__ int token[];   // [block_size] rows by slot, [block_size] slots that get one
   __shared__ int s_later, s_n;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  chain_wait();
+  chain_next();
   const int t = blockIdx.x, tokens = (int)a.tokens;
   const int64_t slot = a.slots[t], before = t > 0 ? a.slots[t - 1] : -1;
   if (slot < 0) return;
@@ -264,6 +266,8 @@ struct Runs { int2* blocks; int* number; int2* list; };
 
 __global__ void __launch_bounds__(256)
 kv8_runs_kernel(const WriteArgs a, const Runs r) {
+  chain_wait();
+  chain_next();
   const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (t >= a.tokens) return;
   const int64_t slot = a.slots[t];
@@ -283,6 +287,8 @@ template <typename T, int D, bool kAligned>
 __global__ void __launch_bounds__(kThreads, 4)
 kv8_write_runs_kernel(const WriteArgs a, const Runs r) {
   extern __shared__ int tokens[];   // [warps][2 * block_size], for blocks of several runs
+  chain_wait();
+  chain_next();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, which = blockIdx.y * (kThreads / 32) + warp;
   if (which >= 2 * a.heads) return;
   const int plane = which >= a.heads, head = plane ? which - a.heads : which, number = *r.number, step = gridDim.x;
@@ -336,23 +342,21 @@ template <typename T, int D, bool kAligned>
 int launch_write(const WriteArgs& a, void* workspace, cudaStream_t stream) {
   const int slices = (2 * a.heads + kThreads / 32 - 1) / (kThreads / 32);
   if (a.tokens <= kScanRows) {
-    kv8_write_kernel<T, D, kAligned><<<dim3((unsigned)a.tokens, slices), kThreads, 2 * a.block_size * sizeof(int), stream>>>(a);
-    return launch_status("kv8_write_kernel");
+    return launch_chained("kv8_write_kernel", kv8_write_kernel<T, D, kAligned>, dim3((unsigned)a.tokens, slices), kThreads,
+                          2 * a.block_size * sizeof(int), stream, a);
   }
   int* base = static_cast<int*>(workspace) + kPlanWords;   // the attention calls' header stays as it is
   int2* blocks = reinterpret_cast<int2*>(base + 2);
   const Runs r{blocks, base, blocks + a.num_blocks};
   APS_CUDA(cudaMemsetAsync(base, 0, 2 * sizeof(int) + (size_t)a.num_blocks * sizeof(int2), stream));
-  kv8_runs_kernel<<<(unsigned)((a.tokens + 255) / 256), 256, 0, stream>>>(a, r);
-  int st = launch_status("kv8_runs_kernel");
+  int st = launch_chained("kv8_runs_kernel", kv8_runs_kernel, (unsigned)((a.tokens + 255) / 256), 256, 0, stream, a, r);
   if (st != APS_OK) return st;
   const size_t smem = (size_t)kThreads / 32 * 2 * a.block_size * sizeof(int);
   if (smem > 48 * 1024)
     APS_CUDA(cudaFuncSetAttribute(kv8_write_runs_kernel<T, D, kAligned>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   int64_t x = ((int64_t)sm_count() * 4 + slices - 1) / slices;   // four CTAs per SM
   if (x > a.tokens) x = a.tokens;
-  kv8_write_runs_kernel<T, D, kAligned><<<dim3((unsigned)x, slices), kThreads, smem, stream>>>(a, r);
-  return launch_status("kv8_write_runs_kernel");
+  return launch_chained("kv8_write_runs_kernel", kv8_write_runs_kernel<T, D, kAligned>, dim3((unsigned)x, slices), kThreads, smem, stream, a, r);
 }
 
 template <typename T>
