@@ -67,6 +67,8 @@ PROTOTYPES = {
                               [c_float, c_int, c_void_p]),
     "aps_kv8_write_workspace_bytes": (c_size_t, [c_int64, c_int64]),
     "aps_kv8_write": (c_int, [c_void_p] * 7 + [c_int64] + [c_int] * 3 + [c_int64] * 5 + [c_void_p, c_size_t, c_int, c_void_p]),
+    "aps_kv8_decode_step": (c_int, [c_void_p] * 9 + [c_int64] + [c_void_p] * 2 + [c_int] * 5 + [c_int64] * 7 +
+                            [c_float, c_void_p, c_size_t, c_int, c_void_p]),
     "aps_kv8_attention_workspace_bytes": (c_size_t, [c_int, c_int64] + [c_int] * 4),
     "aps_kv8_attention": (c_int, [c_void_p] * 9 + [c_int, c_int64] + [c_int] * 5 + [c_int64] * 5 +
                           [c_float, c_void_p, c_size_t, c_int, c_void_p]),
@@ -198,9 +200,11 @@ _nothing = _Nothing()
 
 def on_device(device: torch.device):
     """``torch.cuda.device(device)``, which costs a few microseconds a call, only where it is not current already."""
-    return _nothing if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _nothing if device.index == _current_device() else torch.cuda.device(device)
 
 
+# of a process whose CUDA side is up, as it is where there are CUDA tensors; torch.cuda.current_device looks after that first
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 

@@ -18,6 +18,7 @@ Two ways in:
 from __future__ import annotations
 
 from dataclasses import dataclass, replace
+from functools import lru_cache
 from typing import Any, Dict, List, Optional, Tuple, Type
 
 import torch
@@ -195,20 +196,30 @@ def paged_prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_c
                        scale, k_scale, v_scale, out, workspace)
 
 
+@lru_cache(maxsize=256)
+def _fp8_scratch_bytes(batch: int, rows: int, max_blocks: int, block_size: int, heads: int, head_size: int) -> int:
+    return N.lib().aps_kv8_attention_workspace_bytes(batch, rows, max_blocks, block_size, heads, head_size)
+
+
 def _attend_fp8(op, query, key_cache, value_cache, block_tables, starts, seq_lens, max_rows, scale, k_scale, v_scale, out, workspace):
     ops.check_fp8_cache(op, key_cache, value_cache, k_scale, v_scale)
     dev = N.require_cuda(query, key_cache, value_cache, block_tables, starts, seq_lens, k_scale, v_scale, out, workspace)
     nb, bs, h, d = key_cache.shape
-    if query.dim() != 2 or query.shape[1] != h * d or query.stride(1) != 1:
-        raise RuntimeError(f"{op}: query must be [T, {h * d}] with contiguous rows")
-    t = query.shape[0]
+    shape, steps, width = query.shape, query.stride(), h * d
+    if len(shape) != 2 or shape[1] != width or steps[1] != 1:
+        raise RuntimeError(f"{op}: query must be [T, {width}] with contiguous rows")
+    t = shape[0]
     if out is None:
         out = torch.empty_like(query, memory_format=torch.contiguous_format)
-    elif out.shape != query.shape or out.dtype != query.dtype or out.stride(1) != 1:
-        raise RuntimeError(f"{op}: out must be like query, with contiguous rows")
+        out_step = width
+    else:
+        if out.shape != shape or out.dtype != query.dtype or out.stride(1) != 1:
+            raise RuntimeError(f"{op}: out must be like query, with contiguous rows")
+        out_step = out.stride(0) if t > 1 else width
     bt = _i32(block_tables, "block_tables")
     sl = _i32(seq_lens, "seq_lens")
-    if bt.dim() != 2 or sl.dim() != 1:
+    tables, lens = bt.shape, sl.shape
+    if len(tables) != 2 or len(lens) != 1:
         raise RuntimeError(f"{op}: block_tables must be [B, max_blocks], seq_lens [B]")
     if starts is None:
         b = t
@@ -217,23 +228,21 @@ def _attend_fp8(op, query, key_cache, value_cache, block_tables, starts, seq_len
         if starts.dim() != 1 or starts.shape[0] < 1 or max_rows < 0:
             raise RuntimeError(f"{op}: query_start_loc must hold a start for every request and the end, max_query_len must not be negative")
         b = starts.shape[0] - 1
-    if bt.shape[0] < b or sl.shape[0] < b:
-        raise RuntimeError(f"{op}: {bt.shape[0]} block tables and {sl.shape[0]} lengths for {b} requests")
+    if tables[0] < b or lens[0] < b:
+        raise RuntimeError(f"{op}: {tables[0]} block tables and {lens[0]} lengths for {b} requests")
     if t == 0 or b == 0:
         return out
-    if bt.shape[1] == 0:
+    if tables[1] == 0:
         raise RuntimeError(f"{op}: block_tables without columns")
-    lib = N.lib()
     with N.on_device(dev):
         if workspace is None:
-            workspace, ws_bytes = _scratch_of(dev, lib.aps_kv8_attention_workspace_bytes(b, t, bt.shape[1], bs, h, d))
+            workspace, ws_bytes = _scratch_of(dev, _fp8_scratch_bytes(b, t, tables[1], bs, h, d))
         else:
             ws_bytes = workspace.numel() * workspace.element_size()
-        N.check(lib.aps_kv8_attention(
+        N.check(N.lib().aps_kv8_attention(
             out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-            bt.data_ptr(), N.ptr(starts), sl.data_ptr(), b, t, max_rows, bt.shape[1], h, d, bs, nb,
-            query.stride(0) if t > 1 else h * d, out.stride(0) if t > 1 else h * d, key_cache.stride(0), k_scale.stride(0), float(scale),
-            workspace.data_ptr(), ws_bytes, N.dtype_enum(query), N.current_stream(dev)))
+            bt.data_ptr(), N.ptr(starts), sl.data_ptr(), b, t, max_rows, tables[1], h, d, bs, nb, steps[0] if t > 1 else width, out_step,
+            key_cache.stride(0), k_scale.stride(0), scale, workspace.data_ptr(), ws_bytes, N.dtype_enum(query), N.current_stream(dev)))
     return out
 
 
@@ -838,6 +847,10 @@ class FlashAttentionImpl:
         the cache holds, the step's own rows included."""
         if m.num_hidden_cache_tokens != 0:
             raise ValueError("hidden-cached requests need a 16-bit or fp32 cache: hidden rows are not held in 8 bits")
+        if m.num_prefill_tokens == 0:
+            output = self._plain_decode_fp8(query, key, value, kv_cache, m, kv_scale)
+            if output is not None:
+                return output
         num_tokens, hidden_size = query.shape
         n_prefill, n_decode = m.num_prefill_tokens, m.num_decode_tokens
         query = query.reshape(-1, self.num_heads * self.head_size)
@@ -863,6 +876,39 @@ class FlashAttentionImpl:
             paged_decode_attention(query[n_prefill:], key_cache, value_cache, decode_meta.block_tables, decode_meta.seq_lens_tensor,
                                    self.scale, out=output[n_prefill:], k_scale=k_scale, v_scale=v_scale)
         return output.view(num_tokens, hidden_size)
+
+    def _plain_decode_fp8(self, query, key, value, kv_cache, m, kv_scale) -> Optional[torch.Tensor]:
+        """The decode tokens of a step in one native call (``aps_kv8_decode_step``), without the views in between; ``None`` for anything
+        that the general path brings into shape or refuses."""
+        tables, lens, slots = m.block_tables, m.seq_lens_tensor, m.slot_mapping
+        n, h, d = m.num_decode_tokens, self.num_heads, self.head_size
+        if (n == 0 or n > 1024 or m.num_prefills != 0 or not isinstance(kv_cache, torch.Tensor) or not isinstance(kv_scale, torch.Tensor)
+                or not isinstance(tables, torch.Tensor) or not isinstance(lens, torch.Tensor) or not isinstance(slots, torch.Tensor)):
+            return None
+        cache, planes, scales, scale_steps, width = kv_cache.shape, kv_cache.stride(), kv_scale.shape, kv_scale.stride(), h * d
+        table, dtype, shape = tables.shape, query.dtype, (n, width)
+        if (len(cache) != 5 or cache[0] < 2 or cache[3:] != (h, d) or planes[2:] != (width, d, 1) or kv_cache.dtype not in ops.FP8_STORAGE
+                or len(scales) != 3 or scales[0] < 2 or scales[1:] != (cache[1], h) or scale_steps[2] != 1 or kv_scale.dtype != torch.float32
+                or len(table) != 2 or table[0] < n or table[1] == 0 or lens.numel() < n or slots.numel() != n
+                or query.shape != shape or key.shape != shape or value.shape != shape or dtype not in N.DTYPE_ENUM
+                or key.dtype != dtype or value.dtype != dtype or slots.dtype != torch.int64 or tables.dtype != torch.int32
+                or lens.dtype != torch.int32 or not (slots.is_contiguous() and tables.is_contiguous() and lens.is_contiguous())):
+            return None
+        q_steps, k_steps, v_steps = query.stride(), key.stride(), value.stride()
+        if q_steps[1] != 1 or k_steps[1] != 1 or v_steps[1] != 1:
+            return None
+        if n == 1:   # a single row has the first stride of whatever it was cut from
+            q_steps = k_steps = v_steps = (width, 1)
+        dev = N.require_cuda(query, key, value, kv_cache, kv_scale, slots, tables, lens)
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
+        kc, ks, lib = kv_cache.data_ptr(), kv_scale.data_ptr(), N.lib()
+        with N.on_device(dev):
+            ws, ws_bytes = _scratch_of(dev, _fp8_scratch_bytes(n, n, table[1], cache[2], h, d))
+            N.check(lib.aps_kv8_decode_step(
+                out.data_ptr(), query.data_ptr(), key.data_ptr(), value.data_ptr(), kc, kc + planes[0], ks, ks + 4 * scale_steps[0],
+                slots.data_ptr(), n, tables.data_ptr(), lens.data_ptr(), n, table[1], h, d, cache[2], cache[1], q_steps[0], k_steps[0],
+                v_steps[0], width, planes[1], scale_steps[1], self.scale, ws.data_ptr(), ws_bytes, N.DTYPE_ENUM[dtype], N.current_stream(dev)))
+        return out
 
     def _plain_decode(self, query, key, value, kv_cache, m) -> Optional[torch.Tensor]:
         """``forward`` for what almost every step of plain serving is, a batch of decode tokens without hidden-cached

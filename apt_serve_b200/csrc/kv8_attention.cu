@@ -279,6 +279,40 @@ extern "C" size_t aps_kv8_attention_workspace_bytes(int batch, int64_t num_rows,
   return part_scratch(num_rows, num_heads, head_size, most);
 }
 
+namespace aps {
+namespace {
+
+// The call as it will run, or what is wrong with it.
+int plan_attention(const Kv8Call& c, void* workspace, size_t workspace_bytes, Way* way, Kv8Parts* a) {
+  const int st = check_call("kv8_attention", c);
+  if (st != APS_OK || c.rows == 0 || c.batch == 0) return st;
+  APS_REQUIRE(c.starts != nullptr || c.rows == c.batch, APS_ERR_SHAPE, "kv8_attention: %lld query rows for %d requests",
+              (long long)c.rows, c.batch);
+  *way = kv8_stream_takes(c) ? kStream : kv8_tiles_take(c) ? kTiles : kRows;
+  const int splits = *way == kStream ? kv8_stream_splits(c) : *way == kTiles ? kv8_tile_splits(c) : row_splits(c);
+  *a = Kv8Parts{static_cast<int*>(workspace), nullptr, nullptr, splits, c.scale * 1.4426950408889634f};
+  const size_t need = part_scratch(c.rows, c.cache.heads, c.cache.head_size, splits);
+  APS_REQUIRE(workspace != nullptr && aligned_to(workspace, 256) && workspace_bytes >= need, APS_ERR_WORKSPACE,
+              "kv8_attention: workspace must be 256-byte aligned and hold %zu bytes (got %zu)", need, workspace_bytes);
+  if (splits > 1) {
+    a->ml = reinterpret_cast<float2*>(a->plan + kPlanWords);
+    a->acc = reinterpret_cast<float*>(static_cast<char*>(workspace) + part_acc_at(c.rows, c.cache.heads, splits));
+  }
+  return APS_OK;
+}
+
+int run_attention(const Kv8Call& c, Way way, const Kv8Parts& a, cudaStream_t stream) {
+  if (c.rows == 0 || c.batch == 0) return APS_OK;
+  switch (c.dtype) {
+    case APS_F32: return attend<float>(c, a, way, stream);
+    case APS_F16: return attend<__half>(c, a, way, stream);
+    default: return attend<__nv_bfloat16>(c, a, way, stream);
+  }
+}
+
+}  // namespace
+}  // namespace aps
+
 extern "C" int aps_kv8_attention(void* out, const void* query, const void* key_cache, const void* value_cache, const float* key_scale,
                                  const float* value_scale, const int32_t* block_tables, const int32_t* query_start_loc,
                                  const int32_t* seq_lens, int batch, int64_t num_rows, int max_query_len, int max_blocks_per_seq,
@@ -290,23 +324,27 @@ extern "C" int aps_kv8_attention(void* out, const void* query, const void* key_c
                    num_heads, head_size, block_size},
                   block_tables, query_start_loc, seq_lens, batch, max_blocks_per_seq, max_query_len, num_rows, query_stride, out_stride,
                   scale, dtype};
-  const int st = check_call("kv8_attention", c);
-  if (st != APS_OK || num_rows == 0 || batch == 0) return st;
-  APS_REQUIRE(query_start_loc != nullptr || num_rows == batch, APS_ERR_SHAPE, "kv8_attention: %lld query rows for %d requests",
-              (long long)num_rows, batch);
-  const Way way = kv8_stream_takes(c) ? kStream : kv8_tiles_take(c) ? kTiles : kRows;
-  Kv8Parts a{static_cast<int*>(workspace), nullptr, nullptr,
-             way == kStream ? kv8_stream_splits(c) : way == kTiles ? kv8_tile_splits(c) : row_splits(c), scale * 1.4426950408889634f};
-  const size_t need = part_scratch(num_rows, num_heads, head_size, a.splits);
-  APS_REQUIRE(workspace != nullptr && aligned_to(workspace, 256) && workspace_bytes >= need, APS_ERR_WORKSPACE,
-              "kv8_attention: workspace must be 256-byte aligned and hold %zu bytes (got %zu)", need, workspace_bytes);
-  if (a.splits > 1) {
-    a.ml = reinterpret_cast<float2*>(a.plan + kPlanWords);
-    a.acc = reinterpret_cast<float*>(static_cast<char*>(workspace) + part_acc_at(num_rows, num_heads, a.splits));
-  }
-  switch (dtype) {
-    case APS_F32: return attend<float>(c, a, way, (cudaStream_t)stream);
-    case APS_F16: return attend<__half>(c, a, way, (cudaStream_t)stream);
-    default: return attend<__nv_bfloat16>(c, a, way, (cudaStream_t)stream);
-  }
+  Way way = kRows;
+  Kv8Parts a{};
+  const int st = plan_attention(c, workspace, workspace_bytes, &way, &a);
+  return st != APS_OK ? st : run_attention(c, way, a, (cudaStream_t)stream);
+}
+
+extern "C" int aps_kv8_decode_step(void* out, const void* query, const void* key, const void* value, void* key_cache, void* value_cache,
+                                   float* key_scale, float* value_scale, const int64_t* slot_mapping, int64_t num_slots,
+                                   const int32_t* block_tables, const int32_t* seq_lens, int batch, int max_blocks_per_seq, int num_heads,
+                                   int head_size, int block_size, int64_t num_blocks, int64_t query_stride, int64_t key_stride,
+                                   int64_t value_stride, int64_t out_stride, int64_t block_stride, int64_t scale_stride, float scale,
+                                   void* workspace, size_t workspace_bytes, int dtype, void* stream) {
+  const Kv8Call c{out, query,
+                  {(const uint8_t*)key_cache, (const uint8_t*)value_cache, key_scale, value_scale, num_blocks, block_stride, scale_stride,
+                   num_heads, head_size, block_size},
+                  block_tables, nullptr, seq_lens, batch, max_blocks_per_seq, 1, batch, query_stride, out_stride, scale, dtype};
+  Way way = kRows;
+  Kv8Parts a{};
+  int st = plan_attention(c, workspace, workspace_bytes, &way, &a);   // before anything is written
+  if (st != APS_OK) return st;
+  st = aps_kv8_write(key, value, key_cache, value_cache, key_scale, value_scale, slot_mapping, num_slots, num_heads, head_size, block_size,
+                     num_blocks, key_stride, value_stride, block_stride, scale_stride, workspace, workspace_bytes, dtype, stream);
+  return st != APS_OK ? st : run_attention(c, way, a, (cudaStream_t)stream);
 }

@@ -13,7 +13,7 @@ from . import _native as N
 
 #: what vLLM calls an e4m3 cache
 FP8_CACHE = ("fp8", "fp8_e4m3")
-_FP8_STORAGE = (torch.float8_e4m3fn, torch.uint8)
+FP8_STORAGE = (torch.float8_e4m3fn, torch.uint8)
 
 
 def check_fp8_cache(op: str, key_cache: torch.Tensor, value_cache: torch.Tensor, k_scale, v_scale) -> None:
@@ -21,16 +21,17 @@ def check_fp8_cache(op: str, key_cache: torch.Tensor, value_cache: torch.Tensor,
     ``[NB, H]``, one for each block and head."""
     if not isinstance(k_scale, torch.Tensor) or not isinstance(v_scale, torch.Tensor):
         raise ValueError(f"{op}: an 8-bit cache needs k_scale and v_scale tensors")
-    if key_cache.dtype not in _FP8_STORAGE or value_cache.dtype != key_cache.dtype:
-        raise ValueError(f"{op}: an 8-bit cache is float8_e4m3fn or uint8 (got {key_cache.dtype}, {value_cache.dtype})")
-    if key_cache.dim() != 4 or value_cache.shape != key_cache.shape:
+    dtype, shape, strides, rows = key_cache.dtype, key_cache.shape, key_cache.stride(), k_scale.stride()
+    if dtype not in FP8_STORAGE or value_cache.dtype != dtype:
+        raise ValueError(f"{op}: an 8-bit cache is float8_e4m3fn or uint8 (got {dtype}, {value_cache.dtype})")
+    if len(shape) != 4 or value_cache.shape != shape:
         raise RuntimeError(f"{op}: the caches must be [blocks, block size, heads, head size], alike for keys and values")
-    nb, bs, h, d = key_cache.shape
-    if key_cache.stride()[1:] != (h * d, d, 1) or value_cache.stride() != key_cache.stride():
+    nb, _, h, d = shape
+    if strides != (strides[0], h * d, d, 1) or value_cache.stride() != strides:
         raise RuntimeError(f"{op}: a cache block must be contiguous, and the two caches' strides alike")
-    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if t.dtype != torch.float32 or t.shape != (nb, h) or t.stride(1) != 1 or t.stride(0) != k_scale.stride(0):
-            raise RuntimeError(f"{op}: {name} must be float32 [{nb}, {h}] with contiguous rows, strides alike")
+    if (k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32 or k_scale.shape != (nb, h) or v_scale.shape != (nb, h)
+            or rows[1] != 1 or v_scale.stride() != rows):
+        raise RuntimeError(f"{op}: k_scale and v_scale must be float32 [{nb}, {h}] with contiguous rows, strides alike")
 
 
 def reshape_and_cache_flash(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
@@ -68,29 +69,29 @@ def reshape_and_cache_flash(key: torch.Tensor, value: torch.Tensor, key_cache: t
             N.dtype_enum(key), N.current_stream(dev)))
 
 
-def _row_stride(t: torch.Tensor) -> int:
-    """Elements from row to row of ``[T, H, D]``; of a single row, whose stride can be anything, its width."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+#: up to so many rows ``aps_kv8_write`` takes no scratch
+_SCAN_ROWS = 1024
 
 
 def _write_fp8(dev, key, value, key_cache, value_cache, slot_mapping, k_scale, v_scale) -> None:
     nb, bs, h, d = key_cache.shape
     if key.dtype != value.dtype:
         raise RuntimeError("reshape_and_cache_flash: dtypes differ")
-    for t in (key, value):
-        if t.dim() != 3 or t.shape[1:] != (h, d) or t.stride(2) != 1 or (h > 1 and t.stride(1) != d):
-            raise RuntimeError(f"reshape_and_cache_flash: key and value must be [T, {h}, {d}] with contiguous token rows")
+    rows, v_rows, steps, v_steps = key.shape, value.shape, key.stride(), value.stride()
+    if (len(rows) != 3 or len(v_rows) != 3 or rows[1] != h or rows[2] != d or v_rows[1] != h or v_rows[2] != d or steps[2] != 1 or v_steps[2] != 1
+            or (h > 1 and (steps[1] != d or v_steps[1] != d))):
+        raise RuntimeError(f"reshape_and_cache_flash: key and value must be [T, {h}, {d}] with contiguous token rows")
     slots = slot_mapping if slot_mapping.is_contiguous() else slot_mapping.contiguous()
-    n, lib = min(slots.numel(), key.shape[0], value.shape[0]), N.lib()
-    workspace, ws_bytes = None, lib.aps_kv8_write_workspace_bytes(n, nb)
-    if ws_bytes:
+    n, lib = min(slots.numel(), rows[0], v_rows[0]), N.lib()
+    workspace, ws_bytes = None, 0
+    if n > _SCAN_ROWS:
         from .attention import _scratch_of
-        workspace, ws_bytes = _scratch_of(dev, ws_bytes)
+        workspace, ws_bytes = _scratch_of(dev, lib.aps_kv8_write_workspace_bytes(n, nb))
     with N.on_device(dev):
         N.check(lib.aps_kv8_write(
             key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-            slots.data_ptr(), n, h, d, bs, nb, _row_stride(key), _row_stride(value), key_cache.stride(0), k_scale.stride(0),
-            N.ptr(workspace), ws_bytes, N.dtype_enum(key), N.current_stream(dev)))
+            slots.data_ptr(), n, h, d, bs, nb, steps[0] if rows[0] > 1 else h * d, v_steps[0] if v_rows[0] > 1 else h * d,
+            key_cache.stride(0), k_scale.stride(0), N.ptr(workspace), ws_bytes, N.dtype_enum(key), N.current_stream(dev)))
 
 
 def prefill_cache_write(key: Optional[torch.Tensor], value: Optional[torch.Tensor],

@@ -462,6 +462,17 @@ int aps_kv8_attention(void* out, const void* query, const void* key_cache, const
                       int64_t out_stride, int64_t block_stride, int64_t scale_stride, float scale, void* workspace,
                       size_t workspace_bytes, int dtype, void* stream);
 
+/*
+ * The two for the decode tokens of a step, row r of key, value and query request r's: aps_kv8_write of num_slots rows, then
+ * aps_kv8_attention of one row per request.  workspace: the larger of what the two take.
+ */
+int aps_kv8_decode_step(void* out, const void* query, const void* key, const void* value, void* key_cache, void* value_cache,
+                        float* key_scale, float* value_scale, const int64_t* slot_mapping, int64_t num_slots,
+                        const int32_t* block_tables, const int32_t* seq_lens, int batch, int max_blocks_per_seq, int num_heads,
+                        int head_size, int block_size, int64_t num_blocks, int64_t query_stride, int64_t key_stride,
+                        int64_t value_stride, int64_t out_stride, int64_t block_stride, int64_t scale_stride, float scale,
+                        void* workspace, size_t workspace_bytes, int dtype, void* stream);
+
 /* ------------------------------------------------------------------------ */
 /* Index tensors                                                             */
 /* ------------------------------------------------------------------------ */
