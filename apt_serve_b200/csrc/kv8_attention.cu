@@ -185,10 +185,10 @@ kv8_combine_kernel(const Kv8Call c, const Kv8Parts a) {
   }
 }
 
-// Parts a row's tokens are cut into: enough CTAs for the GPU, parts of 256 tokens at least.
+// Parts a row's tokens are cut into: enough CTAs for the GPU, parts of 512 tokens at least (joining them takes a launch).
 int row_splits(const Kv8Call& c) {
   const int64_t units = c.rows * c.cache.heads, tokens = (int64_t)c.max_blocks * c.cache.block_size;
-  const int64_t want = ((int64_t)sm_count() * 8 + units - 1) / units, most = (tokens + 255) / 256;
+  const int64_t want = ((int64_t)sm_count() * 8 + units - 1) / units, most = (tokens + 511) / 512;
   const int64_t n = want < most ? want : most;
   return (int)(n < 1 ? 1 : n > kMostParts ? kMostParts : n);
 }

@@ -286,26 +286,19 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_mag
       ok = mbar_wait_warp(smem_u32(&aux.q_full), 0, abort_flag, status, kStatusTileWait, lane) && wait(aux.k_full, 0);
       tc_fence_after();
       if (ok) scores(0, 0);
-      if constexpr (kTiles == 2) {
-        // the second row tile half a turn behind the first: one's exponentials run beside the other's maxima and waits
-        ok = ok && wait(aux.p_full[0], 0);
-        if (ok) scores(1, 0);
-      }
+      if (ok && kTiles == 2) scores(1, 0);
     }
     for (int j = 0; j < n_tiles && ok; ++j) {
-      const bool more = j + 1 < n_tiles;
-      ok = (!more || wait(aux.k_full, j + 1)) && wait(aux.v_full, j);
-      // S of the next key tile before the products that have to wait for this one's weights; its buffer held those of tile j - 1
+      if (j + 1 < n_tiles) {
+        if (!wait(aux.k_full, j + 1) || (j > 0 && !wait(aux.v_empty, j - 1))) { ok = false; break; }
+        tc_fence_after();
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) scores(t, j + 1);
+      }
+      ok = wait(aux.v_full, j);
 #pragma unroll
       for (int t = 0; t < kTiles && ok; ++t) {
-        const bool some = t == 0 || second;
-        if (more) {
-          ok = j == 0 || wait(aux.o_done[t], j - 1);
-          if (!ok) break;
-          tc_fence_after();
-          scores(t, j + 1);
-        }
-        if (some) ok = wait(aux.p_full[t], j);
+        if (t == 0 || second) ok = wait(aux.p_full[t], j);
         if (!ok) break;
         tc_fence_after();
         values(t, j);
@@ -542,12 +535,12 @@ bool kv8_tiles_take(const Kv8Call& c) {
          (c.cache.head_size == 64 || c.cache.head_size == 128) && c.cache.num_blocks > 0 && c.scale >= 1.17549435e-38f && c.scale < 1.70141183e38f && c.batch <= 65535;
 }
 
-// Parts that the tokens of a tile of rows are cut into: enough CTAs for two per SM, four key tiles each at least.
+// Parts that the tokens of a tile of rows are cut into: enough CTAs for two per SM, eight key tiles each at least.
 int kv8_tile_splits(const Kv8Call& c) {
   const int64_t tiles = ((int64_t)c.max_blocks * c.cache.block_size + 63) / 64;
   const int64_t units = (c.rows + kRows - 1) / kRows * c.cache.heads;   // at least
   int64_t n = ((int64_t)sm_count() * 2 + units - 1) / units;
-  if (n > (tiles + 3) / 4) n = (tiles + 3) / 4;
+  if (n > (tiles + 7) / 8) n = (tiles + 7) / 8;
   return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }
 
