@@ -38,9 +38,14 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t codes) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(codes));
   return r;
 }
+// The four of a word, the halves taken apart by the conversion itself.
+__device__ __forceinline__ void e4m3x4_to_f16x4(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(codes));
+}
 // Four numbers of a word as floats.
 __device__ __forceinline__ void e4m3x4_to_float(uint32_t codes, float* f) {
-  const uint32_t lo = e4m3x2_to_f16x2((uint16_t)codes), hi = e4m3x2_to_f16x2((uint16_t)(codes >> 16));
+  uint32_t lo, hi;
+  e4m3x4_to_f16x4(codes, lo, hi);
   const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
   f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
 }

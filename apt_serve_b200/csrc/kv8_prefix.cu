@@ -196,10 +196,7 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_mag
         for (int h = 0; h < 2; ++h) {
           uint32_t x[4];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            x[2 * e] = e4m3x2_to_f16x2((uint16_t)half[h][e]);
-            x[2 * e + 1] = e4m3x2_to_f16x2((uint16_t)(half[h][e] >> 16));
-          }
+          for (int e = 0; e < 2; ++e) e4m3x4_to_f16x4(half[h][e], x[2 * e], x[2 * e + 1]);
           st_shared16(base + (((piece % 4 * 2 + (h ^ odd)) ^ (row & 7)) << 4), x);
         }
       }

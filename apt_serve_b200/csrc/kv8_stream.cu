@@ -221,8 +221,9 @@ kv8_stream_kernel(const Kv8Call c, const Kv8Parts parts, const int part_groups, 
       const uint32_t w[2][4] = {{lo.x, lo.y, lo.z, lo.w}, {hi.x, hi.y, hi.z, hi.w}};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const uint32_t a0 = e4m3x2_to_f16x2((uint16_t)w[0][e]), a1 = e4m3x2_to_f16x2((uint16_t)w[1][e]);
-        const uint32_t a2 = e4m3x2_to_f16x2((uint16_t)(w[0][e] >> 16)), a3 = e4m3x2_to_f16x2((uint16_t)(w[1][e] >> 16));
+        uint32_t a0, a1, a2, a3;
+        e4m3x4_to_f16x4(w[0][e], a0, a2);
+        e4m3x4_to_f16x4(w[1][e], a1, a3);
 #pragma unroll
         for (int q = 0; q < kSets; ++q) mma16816(s[q], a0, a1, a2, a3, qb[q][4 * h + e][0], qb[q][4 * h + e][1]);
       }
@@ -291,8 +292,9 @@ kv8_stream_kernel(const Kv8Call c, const Kv8Parts parts, const int part_groups, 
     for (int i = 0; i < D / 16; ++i) {   // dims 2 i and 2 i + 1 of the lane's
       const uint32_t b0 = __byte_perm(v[0][i / 2], v[1][i / 2], i & 1 ? 0x7362 : 0x5140);
       const uint32_t b1 = __byte_perm(v[2][i / 2], v[3][i / 2], i & 1 ? 0x7362 : 0x5140);
-      const uint32_t a0 = e4m3x2_to_f16x2((uint16_t)b0), a1 = e4m3x2_to_f16x2((uint16_t)(b0 >> 16));
-      const uint32_t a2 = e4m3x2_to_f16x2((uint16_t)b1), a3 = e4m3x2_to_f16x2((uint16_t)(b1 >> 16));
+      uint32_t a0, a1, a2, a3;
+      e4m3x4_to_f16x4(b0, a0, a1);
+      e4m3x4_to_f16x4(b1, a2, a3);
 #pragma unroll
       for (int q = 0; q < kSets; ++q) mma16816(acc[q][i], a0, a1, a2, a3, p[q][0], p[q][1]);
     }
