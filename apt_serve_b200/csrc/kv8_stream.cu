@@ -81,22 +81,27 @@ __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Groups of 16 tokens of a part, at least: 32, or as few as it takes for a warp of every place on the GPU (12 per SM), but 8: a group
-// takes a warp a quarter of a microsecond, joining the parts four or five.  Tables of up to 16 groups are not cut.
-constexpr int64_t kUnits = 148 * 12;
+// Groups of 16 tokens of a part, at least.  A group takes a warp a quarter of a microsecond, joining the parts four or five, so that
+// tables of up to 16 groups are not cut and parts have eight at least.  Where parts of up to 40 fill the GPU once, as many as fill it
+// (a 30 011-token OPT-1.3B context: 26 groups 34 us, 16 37, 48 41); else 16, and 32 where there are many of them (128 OPT-66B tp 8
+// requests: 16 groups 69 us, 32 77; 256 OPT-13B requests 519 and 500).
+constexpr int64_t kUnits = 148 * 16;   // warps on the GPU at a time
 int part_groups(const Kv8Call& c) {
-  const int64_t each = (int64_t)c.max_blocks * c.cache.block_size / 16;
+  const int64_t each = (int64_t)c.max_blocks * c.cache.block_size / 16, units = (int64_t)c.batch * c.cache.heads;
   if (each <= 16) return 16;
-  const int64_t n = each * c.batch * c.cache.heads / kUnits;
-  return (int)(n < 8 ? 8 : n > 32 ? 32 : n);
+  if (units < kUnits) {
+    const int64_t parts = kUnits / units, n = (each + parts - 1) / parts;
+    if (n <= 40) return (int)(n < 8 ? 8 : n);
+  }
+  return each * units < 128 * kUnits ? 16 : 32;
 }
 
-template <int D> __host__ __device__ constexpr int stages() { return D == 128 ? 4 : 6; }   // groups of a warp in shared memory
+template <int D> __host__ __device__ constexpr int stages() { return D == 128 ? 3 : 6; }   // groups of a warp in shared memory
 template <int D> __host__ __device__ constexpr int stage_bytes() { return 2 * 16 * D + 16; }
 
 // kRows: query rows at most, 1, 8 or 16.
 template <typename T, int D, int kRows>
-__global__ void __launch_bounds__(32, kRows == 16 ? 10 : 12)
+__global__ void __launch_bounds__(32, kRows == 16 ? 10 : 16)
 kv8_stream_kernel(const Kv8Call c, const Kv8Parts parts, const int part_groups, const uint32_t blocks_magic, const int vec) {
   constexpr int kCols = D / 64, kPer = D / 8, kStages = stages<D>();   // 64-byte pieces of a row; dims of a lane in V
   constexpr int kSets = kRows == 16 ? 2 : 1, kEach = kRows == 1 ? 1 : 2;   // sets of 8 query rows; rows of a set whose softmax a lane keeps

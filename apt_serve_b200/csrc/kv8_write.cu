@@ -294,15 +294,17 @@ kv8_write_runs_kernel(const WriteArgs a, const Runs r) {
   const int plane = which >= a.heads, head = plane ? which - a.heads : which, number = *r.number, step = gridDim.x;
   for (int at = blockIdx.x; at < number; at += 32 * step) {
     uint32_t left = 0;   // of 32 runs, those for the general form
-    int2 run = r.list[at];
+    // what a run is about comes in two round trips: the next one's block and the one's after that are on their way meanwhile
+    auto run_at = [&](int k) { return k < 32 && at + k * step < number ? r.list[at + k * step] : make_int2(0, 0); };
+    auto block_of = [&](int2 run) { return (uint32_t)run.y / (uint32_t)a.block_size; };
+    int2 now = run_at(0), then = run_at(1), info = r.blocks[block_of(now)];
     for (int k = 0; k < 32 && at + k * step < number; ++k) {
-      const int2 now = run;
-      const uint32_t block = (uint32_t)now.y / (uint32_t)a.block_size;
-      const int2 info = r.blocks[block];
-      if (at + (k + 1) * step < number) run = r.list[at + (k + 1) * step];
+      const int2 after = run_at(k + 2), next_info = r.blocks[block_of(then)];
+      const uint32_t block = block_of(now);
       const int from = now.y - (int)(block * (uint32_t)a.block_size);
       if (info.x != 1 || !write_head<T, D, kAligned>(a, plane, head, BlockRows{block, info.y - now.x + 1, now.x, from, nullptr, nullptr}, lane))
         left |= 1u << k;
+      now = then; then = after; info = next_info;
     }
     for (; left != 0; left &= left - 1) {
       const int2 now = r.list[at + (__ffs(left) - 1) * step];
