@@ -42,28 +42,25 @@ template <typename T, int D> struct RowCfg {
 
 template <typename T, int N> struct alignas(N * sizeof(T)) Pack { T x[N]; };
 
-// The largest magnitude of the rows, and whether any element is not finite; `some` is what has been seen so far.
+// The largest magnitude of what has been seen (`some`, pairs of 16-bit numbers or a float) and of p; NaN does not count.
+template <typename T> struct Magnitude { using Type = float; };
+template <> struct Magnitude<__half> { using Type = __half2; };
+template <> struct Magnitude<__nv_bfloat16> { using Type = __nv_bfloat162; };
 template <typename T, int N>
-__device__ __forceinline__ uint32_t magnitude(const Pack<T, N>& p, uint32_t some) {
-  if constexpr (sizeof(T) == 2) {   // as integers, two at a time: the order of the numbers, infinities and NaN above them all
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(&p);
+__device__ __forceinline__ typename Magnitude<T>::Type magnitude(const Pack<T, N>& p, typename Magnitude<T>::Type some) {
+  if constexpr (sizeof(T) == 2) {
+    const auto* x = reinterpret_cast<const typename Magnitude<T>::Type*>(&p);
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) some = __vmaxu2(some, w[i] & 0x7fff7fffu);
+    for (int i = 0; i < N / 2; ++i) some = __hmax2(some, __habs2(x[i]));
   } else {
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(&p);
 #pragma unroll
-    for (int i = 0; i < N; ++i) some = max(some, w[i] & 0x7fffffffu);
+    for (int i = 0; i < N; ++i) some = fmaxf(some, fabsf(p.x[i]));
   }
   return some;
 }
-template <typename T> __device__ __forceinline__ float magnitude_value(uint32_t some);   // of the larger half
-template <> __device__ __forceinline__ float magnitude_value<float>(uint32_t some) { return __uint_as_float(some); }
-template <> __device__ __forceinline__ float magnitude_value<__half>(uint32_t some) {
-  return __half2float(__ushort_as_half((unsigned short)max(some & 0xffffu, some >> 16)));
-}
-template <> __device__ __forceinline__ float magnitude_value<__nv_bfloat16>(uint32_t some) {
-  return __uint_as_float(max(some & 0xffffu, some >> 16) << 16);
-}
+__device__ __forceinline__ float magnitude_value(float some) { return some; }
+__device__ __forceinline__ float magnitude_value(__half2 some) { return fmaxf(__low2float(some), __high2float(some)); }
+__device__ __forceinline__ float magnitude_value(__nv_bfloat162 some) { return fmaxf(__low2float(some), __high2float(some)); }
 
 // N finite elements times a power of two as e4m3 numbers.
 template <typename T, int N>
@@ -147,7 +144,7 @@ __device__ __forceinline__ void write_any_head(const WriteArgs& a, int plane, in
   if (lane == 0 && s != old) *scale_at = s;
 }
 
-// The same for what almost all blocks get: up to 16 rows, 16 bytes at a time, all of them in registers; finite values, a scale that is a
+// The same for what almost all blocks get: up to 16 rows, 16 bytes at a time, all of them in registers; no infinities, a scale that is a
 // power of two, no other rows to be rounded to it.  False: nothing has been written, the general form has to do it (after the kernel's other
 // heads: between them its registers would be this one's).
 template <typename T, int D, bool kAligned>
@@ -170,13 +167,12 @@ __device__ __forceinline__ bool write_head(const WriteArgs& a, int plane, int he
       x[i] = *p;
     }
   }
-  uint32_t some = 0;
+  typename Magnitude<T>::Type some{};
 #pragma unroll
   for (int i = 0; i < C::kLoads; ++i)
     if (i * C::kRows < b.n) some = magnitude<T, C::kPer>(x[i], some);
-  some = sizeof(T) == 2 ? max(some & 0xffffu, some >> 16) : some;
-  some = __reduce_max_sync(0xffffffffu, some);
-  const float top = magnitude_value<T>(some);
+  // numbers that are not negative are in the order of their bits
+  const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(magnitude_value(some))));
   const bool anew = b.taken(0);
   const float need = e4m3_scale(top), s = anew ? need : fmaxf(old, need), by = 1.f / s;
   if (!(top <= 3.402823466e38f) || (__float_as_uint(s) & 0x7fffffu) != 0 || (!anew && s != old)) return false;
@@ -356,8 +352,8 @@ int launch_write(const WriteArgs& a, void* workspace, cudaStream_t stream) {
   const size_t smem = (size_t)kThreads / 32 * 2 * a.block_size * sizeof(int);
   if (smem > 48 * 1024)
     APS_CUDA(cudaFuncSetAttribute(kv8_write_runs_kernel<T, D, kAligned>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  int64_t x = ((int64_t)sm_count() * 4 + slices - 1) / slices;   // four CTAs per SM
-  if (x > a.tokens) x = a.tokens;
+  int64_t x = (int64_t)sm_count() * 4 / slices;   // four CTAs per SM, and no few more that would run alone in the end
+  x = x < 1 ? 1 : x > a.tokens ? a.tokens : x;
   return launch_chained("kv8_write_runs_kernel", kv8_write_runs_kernel<T, D, kAligned>, dim3((unsigned)x, slices), kThreads, smem, stream, a, r);
 }
 
