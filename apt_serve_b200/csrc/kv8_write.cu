@@ -40,6 +40,9 @@ template <typename T, int D> struct RowCfg {
   static constexpr int kLoads = 16 / kRows * kParts;                             // pieces of 16 rows
 };
 
+// CTAs per SM: a lane's share of 16 rows of 128 takes 32 registers, in fp32 64.
+template <typename T> __host__ __device__ constexpr int run_ctas() { return sizeof(T) == 2 ? 4 : 2; }
+
 template <typename T, int N> struct alignas(N * sizeof(T)) Pack { T x[N]; };
 
 // The largest magnitude of what has been seen (`some`, pairs of 16-bit numbers or a float) and of p; NaN does not count.
@@ -144,9 +147,98 @@ __device__ __forceinline__ void write_any_head(const WriteArgs& a, int plane, in
   if (lane == 0 && s != old) *scale_at = s;
 }
 
-// The same for what almost all blocks get: up to 16 rows, 16 bytes at a time, all of them in registers; no infinities, a scale that is a
-// power of two, no other rows to be rounded to it.  False: nothing has been written, the general form has to do it (after the kernel's other
-// heads: between them its registers would be this one's).
+// 16 rows at a time in registers, 16 bytes of each, blocks of any size (their rows come a second time, from L2), the block's other rows
+// rounded to a larger scale; no infinities, a scale that is a power of two.  False: nothing has been written.
+template <typename T, int D, bool kAligned>
+__device__ __forceinline__ bool write_rows(const WriteArgs& a, int plane, int head, const BlockRows& b, int lane) {
+  using C = RowCfg<T, D>;
+  using P = Pack<T, C::kPer>;
+  constexpr int kWords = C::kPer / 4;
+  if (!kAligned || C::kParts > 1) return false;
+  const int at = lane / C::kLanes, column = lane % C::kLanes * C::kPer;
+  const T* rows = static_cast<const T*>(plane ? a.value : a.key) + (int64_t)head * D + column;
+  const int64_t step = plane ? a.value_stride : a.key_stride;
+  float* scale_at = (plane ? a.value_scale : a.key_scale) + (int64_t)b.block * a.scale_stride + head;
+  const float old = *scale_at;
+  P x[C::kLoads];
+  auto load = [&](int from) {
+#pragma unroll
+    for (int i = 0; i < C::kLoads; ++i) {
+      const int k = from + i * C::kRows + at;
+      if (from + i * C::kRows < b.n) x[i] = *reinterpret_cast<const P*>(rows + (int64_t)(k < b.n ? b.row_of(k) : b.row_of(0)) * step);   // a row twice is no harm
+    }
+  };
+  typename Magnitude<T>::Type some{};
+  const int last = (b.n - 1) / 16 * 16;
+#pragma unroll 1
+  for (int from = 0; from <= last; from += 16) {
+    load(from);
+#pragma unroll
+    for (int i = 0; i < C::kLoads; ++i)
+      if (from + i * C::kRows < b.n) some = magnitude<T, C::kPer>(x[i], some);
+  }
+  // numbers that are not negative are in the order of their bits
+  const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(magnitude_value(some))));
+  const bool anew = b.taken(0);
+  const float need = e4m3_scale(top), s = anew ? need : fmaxf(old, need), by = 1.f / s;
+  if (!(top <= 3.402823466e38f) || (__float_as_uint(s) & 0x7fffffu) != 0) return false;
+  uint8_t* held = (plane ? a.value_cache : a.key_cache) + (int64_t)b.block * a.block_stride + (int64_t)head * D + column;
+  const int64_t held_row = (int64_t)a.heads * D;
+  const bool in_half = std::is_same<T, __half>::value && by >= 6.103515625e-05f && by <= 32768.f;
+#pragma unroll 1
+  for (int from = last; from >= 0; from -= 16) {   // the last 16 are still there
+    if (from < last) load(from);
+#pragma unroll
+    for (int i = 0; i < C::kLoads; ++i) {
+      const int k = from + i * C::kRows + at;
+      if (k < b.n) {
+        uint32_t w[kWords];
+        if constexpr (std::is_same<T, __half>::value) {
+          if (in_half) quantise_half<C::kPer>(x[i], __float2half2_rn(by), w);
+          else quantise<T, C::kPer>(x[i], by, w);
+        } else {
+          quantise<T, C::kPer>(x[i], by, w);
+        }
+        uint32_t* to = reinterpret_cast<uint32_t*>(held + b.slot_of(k) * held_row);
+        if constexpr (kWords == 2) *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+        else to[0] = w[0];
+      }
+    }
+  }
+  if (!anew && s != old) {   // the block's other rows, 16 slots in one round trip
+    const float ratio = old / s;
+#pragma unroll 1
+    for (int from = 0; from < a.block_size; from += 16) {
+      uint32_t w[C::kLoads][kWords];
+#pragma unroll
+      for (int i = 0; i < C::kLoads; ++i) {
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(held + (from + i * C::kRows + at) * held_row);
+#pragma unroll
+        for (int q = 0; q < kWords; ++q) w[i][q] = p[q];
+      }
+#pragma unroll
+      for (int i = 0; i < C::kLoads; ++i) {
+        const int o = from + i * C::kRows + at;
+        if (b.taken(o)) continue;
+        uint32_t* to = reinterpret_cast<uint32_t*>(held + o * held_row);
+#pragma unroll
+        for (int q = 0; q < kWords; ++q) {
+          float y[4];
+          e4m3x4_to_float(w[i][q], y);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] *= ratio;
+          to[q] = float4_to_e4m3x4(y);
+        }
+      }
+    }
+  }
+  if (lane == 0 && s != old) *scale_at = s;
+  return true;
+}
+
+// For what almost all blocks get: up to 16 rows, 16 bytes at a time, all of them in registers; no infinities, a scale that is a power of
+// two, no other rows to be rounded to it.  False: nothing has been written, one of the forms above has to do it (after the kernel's other
+// heads: between them its registers would be this one's; in one function with the form above 24 OPT-13B prompts took 158 us, so 125).
 template <typename T, int D, bool kAligned>
 __device__ __forceinline__ bool write_head(const WriteArgs& a, int plane, int head, const BlockRows& b, int lane) {
   using C = RowCfg<T, D>;
@@ -177,7 +269,7 @@ __device__ __forceinline__ bool write_head(const WriteArgs& a, int plane, int he
   const float need = e4m3_scale(top), s = anew ? need : fmaxf(old, need), by = 1.f / s;
   if (!(top <= 3.402823466e38f) || (__float_as_uint(s) & 0x7fffffu) != 0 || (!anew && s != old)) return false;
   uint8_t* held = (plane ? a.value_cache : a.key_cache) + (int64_t)b.block * a.block_stride + (int64_t)head * D + column;
-  const int held_row = a.heads * D;
+  const int64_t held_row = (int64_t)a.heads * D;
   const bool in_half = std::is_same<T, __half>::value && by >= 6.103515625e-05f && by <= 32768.f;
 #pragma unroll
   for (int i = 0; i < C::kLoads; ++i) {
@@ -213,7 +305,7 @@ __device__ __forceinline__ int list_rows(const int* token, int* slots, int block
 
 // ---- few rows: one CTA per (row, some heads); the CTAs of the first row of a block do the block ----
 template <typename T, int D, bool kAligned>
-__global__ void __launch_bounds__(kThreads, 4)
+__global__ void __launch_bounds__(kThreads, run_ctas<T>())
 kv8_write_kernel(const WriteArgs a) {
   extern __shared__ int token[];   // [block_size] rows by slot, [block_size] slots that get one
   __shared__ int s_later, s_n;
@@ -252,7 +344,8 @@ kv8_write_kernel(const WriteArgs a) {
   if (u >= 2 * a.heads) return;
   const int plane = u >= a.heads, head = plane ? u - a.heads : u;
   const BlockRows b{block, s_n, 0, 0, slots, token};
-  if (!write_head<T, D, kAligned>(a, plane, head, b, lane)) write_any_head<T, D>(a, plane, head, b, lane);
+  if (!write_head<T, D, kAligned>(a, plane, head, b, lane) && !write_rows<T, D, kAligned>(a, plane, head, b, lane))
+    write_any_head<T, D>(a, plane, head, b, lane);
 }
 
 // ---- many rows ----
@@ -279,8 +372,9 @@ kv8_runs_kernel(const WriteArgs a, const Runs r) {
 }
 
 // Every warp for itself: one head of one plane of one run after the other.
-template <typename T, int D, bool kAligned>
-__global__ void __launch_bounds__(kThreads, 4)
+// kShort: blocks of 16 rows.
+template <typename T, int D, bool kAligned, bool kShort>
+__global__ void __launch_bounds__(kThreads, run_ctas<T>())
 kv8_write_runs_kernel(const WriteArgs a, const Runs r) {
   extern __shared__ int tokens[];   // [warps][2 * block_size], for blocks of several runs
   chain_wait();
@@ -289,7 +383,7 @@ kv8_write_runs_kernel(const WriteArgs a, const Runs r) {
   if (which >= 2 * a.heads) return;
   const int plane = which >= a.heads, head = plane ? which - a.heads : which, number = *r.number, step = gridDim.x;
   for (int at = blockIdx.x; at < number; at += 32 * step) {
-    uint32_t left = 0;   // of 32 runs, those for the general form
+    uint32_t left = 0;   // of 32 runs, those for the other forms
     // what a run is about comes in two round trips: the next one's block and the one's after that are on their way meanwhile
     auto run_at = [&](int k) { return k < 32 && at + k * step < number ? r.list[at + k * step] : make_int2(0, 0); };
     auto block_of = [&](int2 run) { return (uint32_t)run.y / (uint32_t)a.block_size; };
@@ -298,8 +392,10 @@ kv8_write_runs_kernel(const WriteArgs a, const Runs r) {
       const int2 after = run_at(k + 2), next_info = r.blocks[block_of(then)];
       const uint32_t block = block_of(now);
       const int from = now.y - (int)(block * (uint32_t)a.block_size);
-      if (info.x != 1 || !write_head<T, D, kAligned>(a, plane, head, BlockRows{block, info.y - now.x + 1, now.x, from, nullptr, nullptr}, lane))
-        left |= 1u << k;
+      const BlockRows b{block, info.y - now.x + 1, now.x, from, nullptr, nullptr};
+      bool done = info.x == 1;
+      if (done) done = kShort ? write_head<T, D, kAligned>(a, plane, head, b, lane) : write_rows<T, D, kAligned>(a, plane, head, b, lane);
+      if (!done) left |= 1u << k;
       now = then; then = after; info = next_info;
     }
     for (; left != 0; left &= left - 1) {
@@ -350,11 +446,11 @@ int launch_write(const WriteArgs& a, void* workspace, cudaStream_t stream) {
   int st = launch_chained("kv8_runs_kernel", kv8_runs_kernel, (unsigned)((a.tokens + 255) / 256), 256, 0, stream, a, r);
   if (st != APS_OK) return st;
   const size_t smem = (size_t)kThreads / 32 * 2 * a.block_size * sizeof(int);
-  if (smem > 48 * 1024)
-    APS_CUDA(cudaFuncSetAttribute(kv8_write_runs_kernel<T, D, kAligned>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  int64_t x = (int64_t)sm_count() * 4 / slices;   // four CTAs per SM, and no few more that would run alone in the end
+  auto kernel = a.block_size == 16 ? kv8_write_runs_kernel<T, D, kAligned, true> : kv8_write_runs_kernel<T, D, kAligned, false>;
+  if (smem > 48 * 1024) APS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  int64_t x = (int64_t)sm_count() * run_ctas<T>() / slices;   // and no few more that would run alone in the end
   x = x < 1 ? 1 : x > a.tokens ? a.tokens : x;
-  return launch_chained("kv8_write_runs_kernel", kv8_write_runs_kernel<T, D, kAligned>, dim3((unsigned)x, slices), kThreads, smem, stream, a, r);
+  return launch_chained("kv8_write_runs_kernel", kernel, dim3((unsigned)x, slices), kThreads, smem, stream, a, r);
 }
 
 template <typename T>
