@@ -5,7 +5,10 @@ tokens, the fp32 score of a token is off by at most (D + 2) 2^-24 S, its weight 
 rounding of it to fp16, a sum of n weights or products by n 2^-24: with size = sum_t p_t |v_t|, all of it twice over (numerator and
 denominator)
     |x - y| <= u |y| + (2 (D + 2) 2^-24 S + 2 n 2^-24 + w) size,   w = 2^-11, fp32: 2^-22 (the exponential),
-and 2^-25 for fp16 outputs below the normal range."""
+and 2^-25 for fp16 outputs below the normal range.  A weight times its block's value scale is kept so that the largest is 2^7 at least:
+one below 2^-14, fp16's normal range, is off by 2^-25 instead, so the output by
+    2^-25 2^-7 max_t (p_t s_t) sum_t |code_t|
+more, which shows where the tokens that have the weight have next to nothing in a dimension."""
 import pytest
 import torch
 
@@ -59,10 +62,10 @@ def same_codes(a, b):
 
 
 def attention_reference(q, k8, v8, ks, vs, tables, starts, lens, scale):
-    """[T, H, D] outputs in 64 bits, sum p |v|, S and n of the rows, NaN where a row belongs to no request."""
+    """[T, H, D] outputs in 64 bits, sum p |v|, S and n of the rows, what small weights add; NaN where a row belongs to no request."""
     t, h, d = q.shape
     bs, most = k8.shape[1], tables.shape[1] * k8.shape[1]
-    out, size = (torch.full((t, h, d), float("nan"), dtype=torch.double, device=DEV) for _ in range(2))
+    out, size, least = (torch.full((t, h, d), float("nan"), dtype=torch.double, device=DEV) for _ in range(3))
     score, count = torch.zeros(t, h, 1, dtype=torch.double, device=DEV), torch.zeros(t, 1, 1, dtype=torch.double, device=DEV)
     for r, n in enumerate(lens):
         a, b = starts[r], starts[r + 1]
@@ -70,27 +73,30 @@ def attention_reference(q, k8, v8, ks, vs, tables, starts, lens, scale):
         ids = tables[r, :-(-n // bs)].long()
         k, v = ((c.view(torch.uint8)[ids].view(E4M3).double() * s[ids].double()[:, None, :, None]).flatten(0, 1)[:n]
                 for c, s in ((k8, ks), (v8, vs)))
+        codes = v8.view(torch.uint8)[ids].view(E4M3).double().abs().flatten(0, 1)[:n]
+        steps = vs[ids].double().repeat_interleave(bs, 0)[:n]
         for i in range(a, b):
             keys = n - (b - 1 - i)
             if keys <= 0:
-                out[i], size[i] = 0.0, 0.0
+                out[i], size[i], least[i] = 0.0, 0.0, 0.0
                 continue
             each = q[i].double()[None] * k[:keys] * scale
             p = torch.softmax(each.sum(2), dim=0)
             out[i] = torch.einsum("kh,khd->hd", p, v[:keys])
             size[i] = torch.einsum("kh,khd->hd", p, v[:keys].abs())
+            least[i] = 2.0 ** -32 * (p * steps[:keys]).amax(0)[:, None] * codes[:keys].sum(0)
             score[i, :, 0] = each.abs().sum(2).amax(0)
             count[i] = keys
-    return out, size, score, count
+    return out, size, score, count, least
 
 
 def check(got, ref, dtype):
-    out, size, score, count = ref
+    out, size, score, count, least = ref
     t, h, d = out.shape
     got = got.double().view(t, h, d)
     w = 2.0 ** -22 if dtype == F32 else 2.0 ** -11
     bound = U[dtype] * out.abs() + (2 * (d + 2) * 2.0 ** -24 * score + 2 * count * 2.0 ** -24 + w) * size
-    bound = bound + (2.0 ** -25 if dtype == F else 0.0) + 1e-300
+    bound = bound + (2.0 ** -25 if dtype == F else 0.0) + (0.0 if dtype == F32 else least) + 1e-300
     bad = ~((got - out).abs() <= bound)
     assert not bad.any(), (int(bad.sum()), bad.nonzero()[0].tolist(), float(((got - out).abs() / bound).max()))
 
@@ -495,3 +501,68 @@ def test_a_layer_serves_requests_from_an_8_bit_cache(h, d, dtype):
     engine.swap_in(torch.tensor([[2, int(tables[1, 0])]]))
     advance([1, 1, 1], None)
     A.raise_on_device_status()
+
+
+def test_padded_decode_batches_and_mixed_ones():
+    """A decode batch padded for a graph (slot -1, length 0) and a batch of prompt chunks and decode tokens, through the backend."""
+    h, d, bs, nb = 3, 64, 16, 40
+    cache, scales = make_cache(nb, bs, h, d, seed=8)
+    impl = A.FlashAttentionImpl(h, d, 0.125, h, None, None, "fp8_e4m3")
+    lens = [40, 17, 0, 0]
+    tables = make_tables([40, 17, 0, 0], bs, nb)
+    slots = torch.tensor([int(tables[0, 2]) * bs + 7, int(tables[1, 1]) * bs, -1, -1], device=DEV)
+    q, (k, v) = query(4, h, d, F), rows_of(4, h, d, F, seed=3)
+    want = [(cache[p].cpu().view(torch.uint8).clone(), scales[p].cpu().clone()) for p in (0, 1)]
+    for p, rows in ((0, k), (1, v)):
+        write_reference(*want[p], rows.cpu(), slots.tolist(), bs)
+    meta = metadata(None, lens, tables, slots, None)
+    got = impl.forward(q, k.reshape(4, -1), v.reshape(4, -1), cache, None, meta, scales)
+    for p in (0, 1):
+        assert same_codes(cache[p], want[p][0]) and torch.equal(scales[p].cpu(), want[p][1])
+    check(got, attention_reference(q.reshape(-1, h, d), cache[0], cache[1], scales[0], scales[1], tables, list(range(5)), lens, 0.125), F)
+    assert (got[2:] == 0).all()
+
+    rows, lens = [30, 5, 1, 1], [50, 5, 33, 17]   # two chunks of prompts, two decode tokens
+    tables = make_tables(lens, bs, nb, seed=4)
+    pos = [(r, p) for r, n in enumerate(rows) for p in range(lens[r] - n, lens[r])]
+    slots = torch.tensor([int(tables[r, p // bs]) * bs + p % bs for r, p in pos], device=DEV)
+    t = len(pos)
+    q, (k, v) = query(t, h, d, B), rows_of(t, h, d, B, seed=5)
+    pre = metadata(rows[:2], lens[:2], tables[:2], slots, True)
+    meta = A.replace(pre, num_prefills=2, num_prefill_tokens=35, num_decode_tokens=2, num_tot_tokens=t, seq_lens=lens,
+                     seq_lens_tensor=torch.tensor(lens, dtype=torch.int32, device=DEV), block_tables=tables, max_decode_seq_len=33,
+                     context_lens_tensor=torch.tensor([20, 0, 32, 16], dtype=torch.int32, device=DEV))
+    got = impl.forward(q, k.reshape(t, -1), v.reshape(t, -1), cache, None, meta, scales)
+    ref = attention_reference(q.reshape(-1, h, d), cache[0], cache[1], scales[0], scales[1], tables, [0, 30, 35, 36, 37], lens, 0.125)
+    check(got, ref, B)
+
+
+def test_what_the_backend_refuses():
+    h, d, bs = 2, 64, 16
+    cache, scales = make_cache(8, bs, h, d)
+    impl = A.FlashAttentionImpl(h, d, 0.125, h, None, None, "fp8")
+    tables = make_tables([20], bs, 8)
+    slots = torch.tensor([int(tables[0, 1]) * bs + 3], device=DEV)
+    q, (k, v) = query(1, h, d, F), rows_of(1, h, d, F, seed=1)
+    meta = metadata(None, [20], tables, slots, None)
+    with pytest.raises(ValueError, match="kv_scale"):
+        impl.forward(q, k.reshape(1, -1), v.reshape(1, -1), cache, None, meta)
+    with pytest.raises(RuntimeError, match="float32"):
+        impl.forward(q, k.reshape(1, -1), v.reshape(1, -1), cache, None, meta, scales.double())
+    with pytest.raises(ValueError, match="float8_e4m3fn or uint8"):
+        impl.forward(q, k.reshape(1, -1), v.reshape(1, -1), cache.view(E4M3).half(), None, meta, scales)
+    with pytest.raises(AssertionError, match="kv_scale"):
+        A.FlashAttentionImpl(h, d, 0.125, h, None, None, "auto").forward(q, k.reshape(1, -1), v.reshape(1, -1), cache.half(), None, meta, scales)
+
+
+@pytest.mark.parametrize("rows,dtype", [(1, F), (1, F32), (7, B), (12, F), (40, B), (200, F)])
+def test_rows_of_unaligned_tensors(rows, dtype):
+    """Query and output rows that no vector load takes."""
+    lens, bs, h, d = [260, 300], 16, 3, 64
+    cache, scales = make_cache(40, bs, h, d)
+    tables = make_tables(lens, bs, 40)
+    starts = [0, rows, 2 * rows]
+    wide = torch.randn(2 * rows, h * d + 5, device=DEV).to(dtype)
+    q, out = wide[:, 3:3 + h * d], torch.zeros(2 * rows, h * d + 3, dtype=dtype, device=DEV)[:, 1:1 + h * d]
+    run_prefix(q, cache, scales, tables, starts, lens, 0.1, out=out)
+    check(out, attention_reference(q.reshape(-1, h, d), cache[0], cache[1], scales[0], scales[1], tables, starts, lens, 0.1), dtype)
