@@ -172,6 +172,16 @@ def require_cuda(*tensors: torch.Tensor) -> torch.device:
     return dev
 
 
+def same_device(first: torch.Tensor, *others: torch.Tensor) -> torch.device:
+    """``require_cuda`` of tensors that are all there, in half the time."""
+    index = first.get_device()   # -1 on the CPU
+    for t in others:
+        if t.get_device() != index:
+            index = -1
+            break
+    return first.device if index >= 0 else require_cuda(first, *others)
+
+
 def ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 

@@ -203,7 +203,10 @@ def _fp8_scratch_bytes(batch: int, rows: int, max_blocks: int, block_size: int, 
 
 def _attend_fp8(op, query, key_cache, value_cache, block_tables, starts, seq_lens, max_rows, scale, k_scale, v_scale, out, workspace):
     ops.check_fp8_cache(op, key_cache, value_cache, k_scale, v_scale)
-    dev = N.require_cuda(query, key_cache, value_cache, block_tables, starts, seq_lens, k_scale, v_scale, out, workspace)
+    if starts is None and out is None and workspace is None:
+        dev = N.same_device(query, key_cache, value_cache, block_tables, seq_lens, k_scale, v_scale)
+    else:
+        dev = N.require_cuda(query, key_cache, value_cache, block_tables, starts, seq_lens, k_scale, v_scale, out, workspace)
     nb, bs, h, d = key_cache.shape
     shape, steps, width = query.shape, query.stride(), h * d
     if len(shape) != 2 or shape[1] != width or steps[1] != 1:
@@ -899,7 +902,7 @@ class FlashAttentionImpl:
             return None
         if n == 1:   # a single row has the first stride of whatever it was cut from
             q_steps = k_steps = v_steps = (width, 1)
-        dev = N.require_cuda(query, key, value, kv_cache, kv_scale, slots, tables, lens)
+        dev = N.same_device(query, key, value, kv_cache, kv_scale, slots, tables, lens)
         out = torch.empty_like(query, memory_format=torch.contiguous_format)
         kc, ks, lib = kv_cache.data_ptr(), kv_scale.data_ptr(), N.lib()
         with N.on_device(dev):

@@ -50,7 +50,10 @@ def reshape_and_cache_flash(key: torch.Tensor, value: torch.Tensor, key_cache: t
         check_fp8_cache("reshape_and_cache_flash", key_cache, value_cache, k_scale, v_scale)
     elif kv_cache_dtype != "auto":  # aptserve_flash_attn.py:311-312: no other cache here
         raise ValueError(f"kv_cache_dtype {kv_cache_dtype!r} is not supported")
-    dev = N.require_cuda(key, value, key_cache, value_cache, slot_mapping, *((k_scale, v_scale) if kv_cache_dtype != "auto" else ()))
+    if kv_cache_dtype != "auto":
+        dev = N.same_device(key, value, key_cache, value_cache, slot_mapping, k_scale, v_scale)
+    else:
+        dev = N.require_cuda(key, value, key_cache, value_cache, slot_mapping)
     if slot_mapping.dtype != torch.int64:
         raise RuntimeError("slot_mapping must be int64")
     if kv_cache_dtype != "auto":
