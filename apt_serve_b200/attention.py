@@ -4,12 +4,14 @@ reference's ``additional_designs/attention/backends/aptserve_flash_attn.py``
 and ``additional_designs/attention/aptserve_layer.py`` (``Attention``), so the
 reference's model code, cache engine and model runner can call it unchanged.
 
-Two ways in:
+Ways in:
 
 * ``FlashAttentionImpl.forward`` keeps the reference's argument list and its op
   sequence (cache-write branch selection of aptserve_flash_attn.py:331-387,
   decode attention of :449-475); each op behind it is one of this package's
   kernels.
+* With ``kv_cache_dtype="fp8"`` it works over a K/V cache held in 8 bits with a scale per block and head
+  (``paged_decode_attention`` and ``paged_prefix_attention`` with ``k_scale`` / ``v_scale``).
 * ``hybrid_decode_attention`` / ``FlashAttentionImpl.forward_hybrid_decode`` is
   the fused call: K/V requests stream their private K/V blocks, hidden requests
   are re-projected from their hidden blocks inside the kernel, and neither the
@@ -96,8 +98,8 @@ def raise_on_device_status(workspace: Optional[torch.Tensor] = None,
     per-device workspace of ``device``) left a non-zero status word: 1..7 = a bounded wait
     of one of its kernels ran out and the call's output is NaN, 8 = K/V-cached
     requests in a batch that was given no K/V cache; or if the operations without a workspace left one on the
-    device: a cache write that was not finished, metadata that points outside its tensors, prompt attention
-    that was not finished (rows of NaN).
+    device: a cache write that was not finished, metadata or slots (of an 8-bit cache) that point outside
+    their tensors, prompt attention that was not finished (rows of NaN).
     Synchronises the current stream, so call it where a synchronisation is cheap (once per engine
     step, beside the sampler's device-to-host copy), not per layer."""
     if workspace is not None:
@@ -114,7 +116,7 @@ def raise_on_device_status(workspace: Optional[torch.Tensor] = None,
     code = cache_ops_status(dev)
     if code != 0:
         what = ("a bounded device-side wait of a cache write ran out; rows are missing in the cache" if code == 1 else
-                "decode metadata pointed outside its tensors; the requests concerned were left out of the step" if code == 2 else
+                "decode metadata pointed outside its tensors, or slots outside an 8-bit cache; the requests or rows concerned were left out" if code == 2 else
                 "a bounded device-side wait of the prompts' attention ran out; the rows concerned were filled with NaN")
         raise RuntimeError(f"aptserve_b200: cache operations status {code}: {what}")
 
@@ -191,7 +193,8 @@ def paged_prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_c
     """Attention of several new tokens per request over its whole context in an 8-bit cache, the new tokens' own rows included (a chunk of
     a prompt behind a cached prefix, drafted tokens to be verified): rows ``query_start_loc[r] ... query_start_loc[r + 1]`` (int32
     ``[B + 1]``, at most ``max_query_len`` each) of ``query [T, H*D]`` are the last of request ``r``'s ``seq_lens[r]`` tokens, each
-    attends to the tokens up to itself -> ``[T, H*D]``.  Rows that belong to no request are left as they are in ``out``."""
+    attends to the tokens up to itself -> ``[T, H*D]``.  Rows that belong to no request are left as they are in ``out``; rows of a request
+    beyond ``max_query_len`` are not computed."""
     return _attend_fp8("paged_prefix_attention", query, key_cache, value_cache, block_tables, query_start_loc, seq_lens, max_query_len,
                        scale, k_scale, v_scale, out, workspace)
 

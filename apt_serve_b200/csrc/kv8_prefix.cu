@@ -1,6 +1,7 @@
 // Several query rows per request over the 8-bit cache (kv8_common.cuh), fp16 / bf16 queries, head sizes 64 and 128.
 //
-// One CTA per (128 query rows of a request, head, part of the tokens), two CTAs per SM, key tiles of 64 tokens up to the diagonal:
+// One CTA per (128 query rows of a request, head, part of the tokens), two CTAs per SM; requests of more than 128 rows: one CTA per SM with
+// two row tiles, which share the keys and values that it turns into fp16.  Key tiles of 64 tokens up to the diagonal:
 //   four warps turn the tile's codes into fp16 on their way from the cache to shared memory (every e4m3 number is an fp16 number)
 //   S = Q K^T   tcgen05, M = 128 rows, N = 64 tokens, both operands K-major in shared memory, S in one of two buffers of tensor memory
 //   a thread per query row turns its row of S into weights, in fp16 over S
@@ -11,6 +12,13 @@
 // of small values that has all the weight fills fp16's range like any other.  O stays in tensor memory and is rescaled only when R has
 // grown by more than 2^8.  The output is O 2^(R - m) / l.
 // bf16 queries become fp16 with a power of two for each row, which leaves 2^-40 of the row's largest element.
+//
+// Measured on one B200: 500 new tokens each of six OPT-13B requests behind 1500 (83 GFLOP) 184 us, 2048 of a 16 001-token OPT-1.3B document
+// (251 GFLOP) 528.  A pair of row tiles takes 1900 cycles a key tile where its exponentials take 1024 (16 a cycle and SM), the products
+// 640 (D = 64) to 1280: the softmax warps of both tiles wait, take maxima and exponentials at the same time, and S of the tile after next
+// waits for this one's P V.  Tried, chunks / document, us (183 / 517 to 185 / 528 without): key tiles of 128 with one S 270 / 785; the second
+// row tile held back by half a turn 196 / 563; two threads per row 200 / 569; a quarter of the exponentials as polynomials 194 / 578; three
+// stages of K and V 191 / 544; one row tile per CTA for long requests too 205 / 561.
 #include "kv8_common.cuh"
 #include "sm100.cuh"
 

