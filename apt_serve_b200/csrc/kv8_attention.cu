@@ -185,6 +185,48 @@ kv8_combine_kernel(const Kv8Call c, const Kv8Parts a) {
   }
 }
 
+// A few parts: one warp per (query row, head), all loads at once (256 OPT-13B requests of four parts: 15 us with the kernel above).
+constexpr int kFewParts = 8;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(256)
+kv8_combine_few_kernel(const Kv8Call c, const Kv8Parts a) {
+  constexpr int kPer = D / 32;
+  chain_wait();
+  chain_next();
+  const int lane = threadIdx.x & 31;
+  const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (unit >= c.rows * c.cache.heads) return;
+  const int64_t t = unit / c.cache.heads, h = unit % c.cache.heads;
+  struct alignas(kPer * 4 > 16 ? 16 : kPer * 4) Piece { float x[kPer]; };
+  float2 ml[kFewParts];
+  Piece y[kFewParts];
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kFewParts; ++i) {
+    ml[i] = i < a.splits ? a.ml[unit * a.splits + i] : make_float2(-INFINITY, 0.f);
+    if (i < a.splits) y[i] = *reinterpret_cast<const Piece*>(a.acc + (unit * a.splits + i) * D + lane * kPer);
+    top = fmaxf(top, ml[i].x);
+  }
+  int req, keys;
+  if (!kv8_find_row(c, t, req, keys)) return;
+  const float ref = top == -INFINITY ? 0.f : top;
+  float sum = 0.f, x[kPer];
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) x[e] = 0.f;
+#pragma unroll
+  for (int i = 0; i < kFewParts; ++i) {
+    if (ml[i].x == -INFINITY) continue;   // a part without tokens has no acc
+    const float w = exp2f(ml[i].x - ref);
+    sum = fmaf(w, ml[i].y, sum);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) x[e] = fmaf(w, y[i].x[e], x[e]);
+  }
+  T* out = static_cast<T*>(c.out) + t * c.out_stride + h * D + lane * kPer;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) out[e] = Elem<T>::from_float(keys == 0 ? 0.f : x[e] / sum);
+}
+
 // Parts a row's tokens are cut into: enough CTAs for the GPU, parts of 512 tokens at least (joining them takes a launch).
 int row_splits(const Kv8Call& c) {
   const int64_t units = c.rows * c.cache.heads, tokens = (int64_t)c.max_blocks * c.cache.block_size;
@@ -207,6 +249,15 @@ int launch_parts_combine(const Kv8Call& c, const Kv8Parts& a, cudaStream_t strea
   if (a.splits == 1) return APS_OK;
   const int64_t grid = c.rows * c.cache.heads;
   APS_REQUIRE(grid < (int64_t(1) << 31), APS_ERR_SHAPE, "kv8_attention: too many rows");
+  if (a.splits <= kFewParts) {
+    const unsigned few = (unsigned)((grid + 7) / 8);
+    switch (c.cache.head_size) {
+      case 32: return launch_chained("kv8_combine_few_kernel", kv8_combine_few_kernel<T, 32>, few, 256, 0, stream, c, a);
+      case 64: return launch_chained("kv8_combine_few_kernel", kv8_combine_few_kernel<T, 64>, few, 256, 0, stream, c, a);
+      case 128: return launch_chained("kv8_combine_few_kernel", kv8_combine_few_kernel<T, 128>, few, 256, 0, stream, c, a);
+      default: return launch_chained("kv8_combine_few_kernel", kv8_combine_few_kernel<T, 256>, few, 256, 0, stream, c, a);
+    }
+  }
   switch (c.cache.head_size) {
     case 32: return launch_chained("kv8_combine_kernel", kv8_combine_kernel<T, 32>, (unsigned)grid, 128, 0, stream, c, a);
     case 64: return launch_chained("kv8_combine_kernel", kv8_combine_kernel<T, 64>, (unsigned)grid, 128, 0, stream, c, a);

@@ -205,6 +205,7 @@ kv8_stream_kernel(const Kv8Call c, const Kv8Parts parts, const int part_groups, 
     }
   }
 
+  const bool both = kSets == 2 && n_rows > 8;   // most requests of a batch can have fewer rows than the largest
   // columns 2 j, 2 j + 1 of a set are the lane's query rows
   float acc[kSets][D / 16][4];   // dims' rows g, g, g + 8, g + 8
 #pragma unroll
@@ -234,7 +235,8 @@ kv8_stream_kernel(const Kv8Call c, const Kv8Parts parts, const int part_groups, 
         e4m3x4_to_f16x4(w[0][e], a0, a2);
         e4m3x4_to_f16x4(w[1][e], a1, a3);
 #pragma unroll
-        for (int q = 0; q < kSets; ++q) mma16816(s[q], a0, a1, a2, a3, qb[q][4 * h + e][0], qb[q][4 * h + e][1]);
+        for (int q = 0; q < kSets; ++q)
+          if (q == 0 || both) mma16816(s[q], a0, a1, a2, a3, qb[q][4 * h + e][0], qb[q][4 * h + e][1]);
       }
     }
     const float lv = lg2(scale.y);
@@ -245,7 +247,9 @@ kv8_stream_kernel(const Kv8Call c, const Kv8Parts parts, const int part_groups, 
 #pragma unroll
     for (int q = 0; q < kSets; ++q) {
       float w[2][2] = {{0.f, 0.f}, {0.f, 0.f}};   // [tokens g, g + 8][rows]
-      down[q][1] = 1.f;
+      down[q][0] = down[q][1] = 1.f;
+      p[q][0] = p[q][1] = 0u;
+      if (q == 1 && !both) continue;
 #pragma unroll
       for (int e = 0; e < kEach; ++e) {
         float by = coef[q][e] * scale.x, x0 = s[q][e], x1 = s[q][2 + e];
@@ -305,7 +309,8 @@ kv8_stream_kernel(const Kv8Call c, const Kv8Parts parts, const int part_groups, 
       e4m3x4_to_f16x4(b0, a0, a1);
       e4m3x4_to_f16x4(b1, a2, a3);
 #pragma unroll
-      for (int q = 0; q < kSets; ++q) mma16816(acc[q][i], a0, a1, a2, a3, p[q][0], p[q][1]);
+      for (int q = 0; q < kSets; ++q)
+        if (q == 0 || both) mma16816(acc[q][i], a0, a1, a2, a3, p[q][0], p[q][1]);
     }
   };
   for (int k = 0; k < n_groups; ++k) {
