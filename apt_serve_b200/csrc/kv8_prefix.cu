@@ -13,12 +13,13 @@
 // grown by more than 2^8.  The output is O 2^(R - m) / l.
 // bf16 queries become fp16 with a power of two for each row, which leaves 2^-40 of the row's largest element.
 //
-// Measured on one B200: 500 new tokens each of six OPT-13B requests behind 1500 (83 GFLOP) 184 us, 2048 of a 16 001-token OPT-1.3B document
-// (251 GFLOP) 528.  A pair of row tiles takes 1900 cycles a key tile where its exponentials take 1024 (16 a cycle and SM), the products
-// 640 (D = 64) to 1280: the softmax warps of both tiles wait, take maxima and exponentials at the same time, and S of the tile after next
-// waits for this one's P V.  Tried, chunks / document, us (183 / 517 to 185 / 528 without): key tiles of 128 with one S 270 / 785; the second
-// row tile held back by half a turn 196 / 563; two threads per row 200 / 569; a quarter of the exponentials as polynomials 194 / 578; three
-// stages of K and V 191 / 544; one row tile per CTA for long requests too 205 / 561.
+// Measured on one B200: 500 new tokens each of six OPT-13B requests behind 1500 (83 GFLOP) 181 us, 2048 of a 16 001-token OPT-1.3B document
+// (251 GFLOP) 521.  A pair of row tiles takes 1900 cycles a key tile where its exponentials take 1024 (16 a cycle and SM), the products
+// 640 (D = 64) to 1280: a softmax warp is busy for 1700 of them, 1100 in the exponentials, which both tiles take at the same time; issue
+// slots 46 %, special function unit 56 %.  Tried, chunks / document, us: key tiles of 128 with one S 270 / 785 (183 / 517 without, before the
+// copies were tile by tile); beside 185 / 528: the second row tile held back by half a turn 196 / 563, two threads per row 200 / 569, a
+// quarter of the exponentials as polynomials 194 / 578, three stages of K and V 191 / 544, one row tile per CTA for long requests too 205 /
+// 561; a warp for the products of each row tile, with and without that half turn, 180 - 184 / 523.
 #include "kv8_common.cuh"
 #include "sm100.cuh"
 
@@ -159,6 +160,10 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_mag
   auto wait = [&](uint64_t* bars, int tile) {
     return mbar_wait_warp(smem_u32(&bars[tile & 1]), (uint32_t)(tile >> 1) & 1u, abort_flag, status, kStatusTileWait, lane);
   };
+  auto wait_two = [&](uint64_t* a, int i, uint64_t* b, int j) {   // both round trips at once
+    const bool there = mbar_try_wait_addr(smem_u32(&a[i & 1]), (uint32_t)(i >> 1) & 1u) & mbar_try_wait_addr(smem_u32(&b[j & 1]), (uint32_t)(j >> 1) & 1u);
+    return __all_sync(0xffffffffu, there) || (wait(a, i) && wait(b, j));
+  };
   auto arrive = [&](uint64_t* bar) {   // what the warp has written to shared memory is the tensor cores'
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
@@ -264,14 +269,17 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_mag
     constexpr uint32_t o_idesc = mma_idesc(0, 128, D, false) | (1u << 16);   // B is MN-major
     // descriptors' low halves: an offset in shared memory adds its sixteenth
     const uint32_t q_lo = desc_lo(q_at, 16), k_lo = desc_lo(k_at, 16), v_lo = desc_lo(v_at, kSlab);
-    auto scores = [&](int t, int j) {   // S of row tile t and key tile j
+    auto scores = [&](int j) {   // S of key tile j
       if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          tc_mma_cta(tmem + t * 256 + (j & 1) * kKeys, q_lo + (t * kQBytes + k / 4 * kQSlab + k % 4 * 32) / 16, desc_hi(1024, true),
-                     k_lo + (j & 1) * (kTileBytes / 16) + (k / 4 * kSlab + k % 4 * 32) / 16, desc_hi(1024, true), s_idesc, k != 0);
-        tc_commit_cta(smem_u32(&aux.s_full[t][(j & 1)]));
-        if (t == kTiles - 1) tc_commit_cta(smem_u32(&aux.k_empty[j & 1]));
+        for (int t = 0; t < kTiles; ++t) {
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            tc_mma_cta(tmem + t * 256 + (j & 1) * kKeys, q_lo + (t * kQBytes + k / 4 * kQSlab + k % 4 * 32) / 16, desc_hi(1024, true),
+                       k_lo + (j & 1) * (kTileBytes / 16) + (k / 4 * kSlab + k % 4 * 32) / 16, desc_hi(1024, true), s_idesc, k != 0);
+          tc_commit_cta(smem_u32(&aux.s_full[t][j & 1]));
+        }
+        tc_commit_cta(smem_u32(&aux.k_empty[j & 1]));
       }
       __syncwarp();
     };
@@ -290,23 +298,24 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_mag
     if (n_tiles > 0) {
       ok = mbar_wait_warp(smem_u32(&aux.q_full), 0, abort_flag, status, kStatusTileWait, lane) && wait(aux.k_full, 0);
       tc_fence_after();
-      if (ok) scores(0, 0);
-      if (ok && kTiles == 2) scores(1, 0);
+      if (ok) scores(0);
     }
     for (int j = 0; j < n_tiles && ok; ++j) {
-      if (j + 1 < n_tiles) {
-        if (!wait(aux.k_full, j + 1) || (j > 0 && !wait(aux.v_empty, j - 1))) { ok = false; break; }
-        tc_fence_after();
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) scores(t, j + 1);
-      }
-      ok = wait(aux.v_full, j);
-#pragma unroll
-      for (int t = 0; t < kTiles && ok; ++t) {
-        if (t == 0 || second) ok = wait(aux.p_full[t], j);
+      if (j + 1 < n_tiles) {   // S of the next key tile, into the buffer that held the weights of tile j - 1
+        ok = j > 0 ? wait_two(aux.k_full, j + 1, aux.v_empty, j - 1) : wait(aux.k_full, 1);
         if (!ok) break;
         tc_fence_after();
-        values(t, j);
+        scores(j + 1);
+      }
+      ok = wait_two(aux.v_full, j, aux.p_full[0], j);
+      if (!ok) break;
+      tc_fence_after();
+      values(0, j);
+      if constexpr (kTiles == 2) {
+        if (second) ok = wait(aux.p_full[1], j);
+        if (!ok) break;
+        tc_fence_after();
+        values(1, j);
       }
     }
   } else {
