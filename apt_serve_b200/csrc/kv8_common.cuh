@@ -112,6 +112,7 @@ int launch_kv8_stream(const Kv8Call& c, const Kv8Parts& parts, cudaStream_t stre
 // Query rows by tiles of 128 on the tensor cores (kv8_prefix.cu).
 bool kv8_tiles_take(const Kv8Call& c);
 int kv8_tile_splits(const Kv8Call& c);
+int kv8_tile_splits(const Kv8Call& c, int tiles);   // with one or two row tiles per CTA
 int launch_kv8_tiles(const Kv8Call& c, const Kv8Parts& parts, cudaStream_t stream);
 
 bool kv8_supported(int dtype, int head_size);
