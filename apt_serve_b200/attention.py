@@ -49,7 +49,7 @@ def _scratch_of(device: torch.device, need: int) -> Tuple[torch.Tensor, int]:
     ws = _workspaces.get(device)
     if ws is None or ws.numel() < need:
         ws = torch.empty(need, dtype=torch.uint8, device=device)
-        ws[:256].zero_()   # no call has left a status in it (a cache write that takes scratch leaves none)
+        ws[:256].zero_()   # no call has left a status in it
         _workspaces[device] = ws
     return ws, need
 
@@ -868,6 +868,8 @@ class FlashAttentionImpl:
                 raise ValueError("an 8-bit cache needs kv_scale, the [2, blocks, heads] tensor of its scales")
             key_cache, value_cache, k_scale, v_scale = kv_cache[0], kv_cache[1], kv_scale[0], kv_scale[1]
             ops.reshape_and_cache_flash(key, value, key_cache, value_cache, m.slot_mapping, self.kv_cache_dtype, k_scale, v_scale)
+        elif n_decode != 0:
+            raise ValueError("decode tokens need a kv_cache")
         output = torch.empty_like(query, memory_format=torch.contiguous_format)
         if (prefill_meta := m.prefill_metadata) is not None:
             if kv_cache is None or prefill_meta.block_tables is None or prefill_meta.block_tables.numel() == 0:

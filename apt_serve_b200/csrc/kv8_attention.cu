@@ -374,8 +374,8 @@ extern "C" int aps_kv8_attention(void* out, const void* query, const void* key_c
   const Kv8Call c{out, query,
                   {(const uint8_t*)key_cache, (const uint8_t*)value_cache, key_scale, value_scale, num_blocks, block_stride, scale_stride,
                    num_heads, head_size, block_size},
-                  block_tables, query_start_loc, seq_lens, batch, max_blocks_per_seq, max_query_len, num_rows, query_stride, out_stride,
-                  scale, dtype};
+                  block_tables, query_start_loc, seq_lens, batch, max_blocks_per_seq,
+                  max_query_len < num_rows ? max_query_len : (int)num_rows, num_rows, query_stride, out_stride, scale, dtype};
   Way way = kRows;
   Kv8Parts a{};
   const int st = plan_attention(c, workspace, workspace_bytes, &way, &a);

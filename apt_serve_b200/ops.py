@@ -87,10 +87,10 @@ def _write_fp8(dev, key, value, key_cache, value_cache, slot_mapping, k_scale, v
     slots = slot_mapping if slot_mapping.is_contiguous() else slot_mapping.contiguous()
     n, lib = min(slots.numel(), rows[0], v_rows[0]), N.lib()
     workspace, ws_bytes = None, 0
-    if n > _SCAN_ROWS:
-        from .attention import _scratch_of
-        workspace, ws_bytes = _scratch_of(dev, lib.aps_kv8_write_workspace_bytes(n, nb))
     with N.on_device(dev):
+        if n > _SCAN_ROWS:   # of the call's own stream, not the attention calls' scratch: writes may run beside those
+            ws_bytes = lib.aps_kv8_write_workspace_bytes(n, nb)
+            workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         N.check(lib.aps_kv8_write(
             key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
             slots.data_ptr(), n, h, d, bs, nb, steps[0] if rows[0] > 1 else h * d, v_steps[0] if v_rows[0] > 1 else h * d,

@@ -426,6 +426,53 @@ def test_captured_calls_replay_on_another_stream():
         assert torch.equal(out, want) and same_codes(cache, want_c) and torch.equal(scales, want_s)
 
 
+def test_prompts_are_written_beside_attention_on_another_stream_and_captured():
+    """A write of many rows has scratch of its own: attention on another stream is not disturbed, nor is a replay by a later call."""
+    lens, bs, h, d = [3000, 700], 16, 2, 128
+    cache, scales = make_cache(240, bs, h, d)
+    tables, seq, q = make_tables(lens, bs, 240), torch.tensor(lens, dtype=torch.int32, device=DEV), query(2, h, d, F)
+    key, value = rows_of(1500, h, d, F, seed=2)
+    slots = torch.arange(1500, device=DEV)
+
+    def write(c, s):
+        ops.reshape_and_cache_flash(key, value, c[0], c[1], slots, "fp8", s[0], s[1])
+
+    def attend():
+        return A.paged_decode_attention(q, cache[0], cache[1], tables, seq, 0.1, k_scale=scales[0], v_scale=scales[1])
+    before = [make_cache(100, bs, h, d, seed=3) for _ in range(3)]
+    want_c, want_s = before[0]
+    write(want_c, want_s)
+    want, side = attend(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    outs = []
+    for _ in range(8):
+        with torch.cuda.stream(side):
+            write(*before[1])
+        outs.append(attend())
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs) and same_codes(before[1][0], want_c) and torch.equal(before[1][1], want_s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        write(*before[2])
+    key.copy_(rows_of(1500, h, d, F, seed=4)[0])
+    write(want_c, want_s)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert same_codes(before[2][0], want_c) and torch.equal(before[2][1], want_s)
+
+
+@pytest.mark.parametrize("rows", [[3, 1], [30, 200]])
+def test_the_bound_of_a_requests_rows_may_be_far_too_large(rows):
+    lens, bs, h, d = [100, 900], 16, 2, 64
+    cache, scales = make_cache(80, bs, h, d)
+    tables, seq = make_tables(lens, bs, 80), torch.tensor(lens, dtype=torch.int32, device=DEV)
+    starts = torch.tensor([0, rows[0], sum(rows)], dtype=torch.int32, device=DEV)
+    q = query(sum(rows), h, d, F)
+    ref = attention_reference(q.reshape(-1, h, d), cache[0], cache[1], scales[0], scales[1], tables, starts.tolist(), lens, 0.1)
+    for most in (max(rows), 2 ** 20, 2 ** 31 - 1):
+        check(A.paged_prefix_attention(q, cache[0], cache[1], tables, starts, seq, most, 0.1, scales[0], scales[1]), ref, F)
+
+
 class _Fp8:
     cache_dtype, sliding_window = "fp8", None
 

@@ -93,6 +93,15 @@ def test_hidden_cached_requests_are_refused():
         layer.attn.impl.forward(x, x, x, None, None, Meta)
 
 
+def test_decode_tokens_without_a_cache_are_refused():
+    class Meta:
+        num_hidden_cache_tokens, num_decode_tokens, num_prefill_tokens, num_prefills = 0, 2, 0, 0
+        block_tables = seq_lens_tensor = slot_mapping = None
+    x = torch.zeros(2, 128)
+    with pytest.raises(ValueError, match="need a kv_cache"):
+        A.FlashAttentionImpl(2, 64, 1.0, 2, None, None, "fp8").forward(x, x, x, None, None, Meta)
+
+
 def test_cache_engine_moves_the_scales_with_the_blocks():
     engine = CacheEngine(2, 4, 64, 16, 8, 4, E4M3, device="cpu", pin_memory=False, hidden_size=512)
     assert engine.gpu_hidden_cache is None and engine.gpu_cache[0].dtype == E4M3 and engine.gpu_scale[1].shape == (2, 8, 4)
