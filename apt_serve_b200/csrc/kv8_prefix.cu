@@ -13,8 +13,8 @@
 // grown by more than 2^8.  The output is O 2^(R - m) / l.
 // bf16 queries become fp16 with a power of two for each row, which leaves 2^-40 of the row's largest element.
 //
-// Measured on one B200: 500 new tokens each of six OPT-13B requests behind 1500 (83 GFLOP) 181 us, 2048 of a 16 001-token OPT-1.3B document
-// (251 GFLOP) 521.  A pair of row tiles takes 1900 cycles a key tile where its exponentials take 1024 (16 a cycle and SM), the products
+// Measured on one B200: 500 new tokens each of six OPT-13B requests behind 1500 (83 GFLOP) 177 us, 2048 of a 16 001-token OPT-1.3B document
+// (251 GFLOP) 514.  A pair of row tiles takes 1900 cycles a key tile where its exponentials take 1024 (16 a cycle and SM), the products
 // 640 (D = 64) to 1280: a softmax warp is busy for 1700 of them, 1100 in the exponentials, which both tiles take at the same time; issue
 // slots 46 %, special function unit 56 %.  Tried, chunks / document, us: key tiles of 128 with one S 270 / 785 (183 / 517 without, before the
 // copies were tile by tile); beside 185 / 528: the second row tile held back by half a turn 196 / 563, two threads per row 200 / 569, a
@@ -113,9 +113,35 @@ __device__ __forceinline__ void st_shared16(uint32_t addr, const uint32_t* w) {
 
 template <int D, int kTiles> __host__ __device__ constexpr size_t tile_smem() { return 1024 + (size_t)(kTiles * kRows + 4 * kKeys) * D * 2; }
 
+// The CTAs' rows, those with the most tokens first: which of the batch * blocks pairs of a request and kTall of its rows (its last ones first)
+// comes at place `rank`.  Ragged batches end together then: six chunks of 424 ... 670 rows 181 us in the order of the requests, 177 in
+// this one; 2048 rows of a document (the last ones first for all heads, not for each) 527 and 514.
+// More than kSorted pairs keep the requests' order: what the last ones are late by is little of the whole.
+constexpr int kSorted = 256;
+
+template <int kTall>
+__device__ __forceinline__ int longest_first(const Kv8Call& c, int blocks, int rank) {
+  const int pairs = c.batch * blocks;
+  if (pairs > kSorted) return rank;
+  __shared__ int s_tokens[kSorted], s_pair;
+  for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
+    const int req = i / blocks, row0 = (blocks - 1 - i % blocks) * kTall, n = c.starts[req + 1] - c.starts[req];
+    const int ctx = max(0, min(c.seq_lens[req], c.max_blocks * c.cache.block_size));
+    s_tokens[i] = row0 < n ? max(0, ctx - n + min(n, row0 + kTall)) : -1;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
+    int place = 0;
+    for (int k = 0; k < pairs; ++k) place += s_tokens[k] > s_tokens[i] || (s_tokens[k] == s_tokens[i] && k < i);
+    if (place == rank) s_pair = i;
+  }
+  __syncthreads();
+  return s_pair;
+}
+
 template <typename T, int D, int kTiles>
 __global__ void __launch_bounds__((kSoftWarp + 4 * kTiles) * 32, kTiles == 1 ? 2 : 1)
-kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_magic, const int vec) {
+kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const int blocks, const uint32_t blocks_magic, const int vec) {
   constexpr uint32_t kQSlab = kRows * 128, kSlab = kKeys * 128, kQBytes = D / 64 * kQSlab, kTileBytes = D / 64 * kSlab;
   constexpr uint32_t kCols = 256 * kTiles, kO = 128;   // tensor memory of a row tile: S (and P over it), then O
   extern __shared__ uint8_t smem_raw[];
@@ -123,10 +149,10 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const uint32_t blocks_mag
   __shared__ Aux<kTiles> aux;
   chain_wait();
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
-  const int head = blockIdx.y, req = blockIdx.z, splits = parts.splits, split = blockIdx.x % splits;
-  if (blockIdx.x == 0 && head == 0 && req == 0 && threadIdx.x == 0) parts.plan[kPlanStatus] = kStatusOk;
-  const int start = c.starts[req], n_rows = c.starts[req + 1] - start;
-  const int row0 = (int)(gridDim.x / splits - 1 - blockIdx.x / splits) * (kTiles * kRows);    // the rows with the most tokens first
+  const int splits = parts.splits, split = blockIdx.x % splits, head = blockIdx.x / splits % c.cache.heads;
+  const int pair = longest_first<kTiles * kRows>(c, blocks, blockIdx.x / splits / c.cache.heads), req = pair / blocks;
+  if (blockIdx.x == 0 && threadIdx.x == 0) parts.plan[kPlanStatus] = kStatusOk;
+  const int start = c.starts[req], n_rows = c.starts[req + 1] - start, row0 = (blocks - 1 - pair % blocks) * (kTiles * kRows);
   if (row0 >= n_rows) { chain_next(); return; }
   const int bs = c.cache.block_size, ctx = max(0, min(c.seq_lens[req], c.max_blocks * bs));
   const int first = ctx - n_rows + row0;                                 // own position of the CTA's first row
@@ -530,8 +556,10 @@ int launch(const Kv8Call& c, const Kv8Parts& parts, cudaStream_t stream) {
   }
   const int vec = aligned_to(c.query, 16) && aligned_to(c.out, 16) && c.query_stride % 8 == 0 && c.out_stride % 8 == 0;
   const int blocks = (c.max_rows + kTiles * kRows - 1) / (kTiles * kRows);
-  return launch_chained("kv8_tile_kernel", kernel, dim3(blocks * parts.splits, c.cache.heads, c.batch), (kSoftWarp + 4 * kTiles) * 32, smem,
-                        stream, c, parts, kv8_blocks_magic(c.cache.block_size), vec);
+  const int64_t grid = (int64_t)c.batch * blocks * c.cache.heads * parts.splits;
+  APS_REQUIRE(grid < (int64_t(1) << 31), APS_ERR_SHAPE, "kv8_attention: too many rows");
+  return launch_chained("kv8_tile_kernel", kernel, (unsigned)grid, (kSoftWarp + 4 * kTiles) * 32, smem, stream, c, parts, blocks,
+                        kv8_blocks_magic(c.cache.block_size), vec);
 }
 
 // Row tiles per CTA: two save a tenth where they are filled (six chunks of 500 rows 185 us, with one 205); where the requests' average
@@ -553,7 +581,7 @@ int launch_typed(const Kv8Call& c, const Kv8Parts& parts, cudaStream_t stream) {
 bool kv8_tiles_take(const Kv8Call& c) {
   // the maximum is taken of the raw scores: a scale that is not positive would need their minimum
   return c.starts != nullptr && c.max_rows > 1 && (c.dtype == APS_F16 || c.dtype == APS_BF16) &&
-         (c.cache.head_size == 64 || c.cache.head_size == 128) && c.cache.num_blocks > 0 && c.scale >= 1.17549435e-38f && c.scale < 1.70141183e38f && c.batch <= 65535;
+         (c.cache.head_size == 64 || c.cache.head_size == 128) && c.cache.num_blocks > 0 && c.scale >= 1.17549435e-38f && c.scale < 1.70141183e38f;
 }
 
 // Parts that the tokens of a tile of rows are cut into: as many as the GPU takes at a time (a few CTAs more would run alone in the end:
