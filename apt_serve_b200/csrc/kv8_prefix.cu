@@ -19,7 +19,8 @@
 // slots 46 %, special function unit 56 %.  Tried, chunks / document, us: key tiles of 128 with one S 270 / 785 (183 / 517 without, before the
 // copies were tile by tile); beside 185 / 528: the second row tile held back by half a turn 196 / 563, two threads per row 200 / 569, a
 // quarter of the exponentials as polynomials 194 / 578, three stages of K and V 191 / 544, one row tile per CTA for long requests too 205 /
-// 561; a warp for the products of each row tile, with and without that half turn, 180 - 184 / 523.
+// 561; a warp for the products of each row tile, with and without that half turn, 180 - 184 / 523; with D = 64 the queries in tensor memory
+// 515 (514 from shared memory).
 #include "kv8_common.cuh"
 #include "sm100.cuh"
 
