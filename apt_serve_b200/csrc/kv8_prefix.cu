@@ -14,7 +14,7 @@
 // bf16 queries become fp16 with a power of two for each row, which leaves 2^-40 of the row's largest element.
 //
 // Measured on one B200: 500 new tokens each of six OPT-13B requests behind 1500 (83 GFLOP) 177 us, 2048 of a 16 001-token OPT-1.3B document
-// (251 GFLOP) 514.  A pair of row tiles takes 1900 cycles a key tile where its exponentials take 1024 (16 a cycle and SM), the products
+// (251 GFLOP) 514.  A pair of row tiles takes 1900 cycles a key tile (D = 64; 128: 2400) where its exponentials take 1024 (16 a cycle and SM), the products
 // 640 (D = 64) to 1280: a softmax warp is busy for 1700 of them, 1100 in the exponentials, which both tiles take at the same time; issue
 // slots 46 %, special function unit 56 %.  Tried, chunks / document, us: key tiles of 128 with one S 270 / 785 (183 / 517 without, before the
 // copies were tile by tile); beside 185 / 528: the second row tile held back by half a turn 196 / 563, two threads per row 200 / 569, a
