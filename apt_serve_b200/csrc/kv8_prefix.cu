@@ -296,10 +296,12 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const int blocks, const u
     constexpr uint32_t o_idesc = mma_idesc(0, 128, D, false) | (1u << 16);   // B is MN-major
     // descriptors' low halves: an offset in shared memory adds its sixteenth
     const uint32_t q_lo = desc_lo(q_at, 16), k_lo = desc_lo(k_at, 16), v_lo = desc_lo(v_at, kSlab);
+    const int used = kTiles == 2 && soft_warps(1) > 0 ? 2 : 1;   // a second row tile without rows has no products: nobody would wait for them
     auto scores = [&](int j) {   // S of key tile j
       if (elect_one()) {
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
+          if (t >= used) break;
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
             tc_mma_cta(tmem + t * 256 + (j & 1) * kKeys, q_lo + (t * kQBytes + k / 4 * kQSlab + k % 4 * 32) / 16, desc_hi(1024, true),
@@ -317,11 +319,10 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const int blocks, const u
           mma_tmem_a(tmem + t * 256 + kO, tmem + t * 256 + (j & 1) * kKeys + k * 8, v_lo + (j & 1) * (kTileBytes / 16) + k * 128,
                      desc_hi(1024, true), o_idesc, j > 0 || k != 0);
         tc_commit_cta(smem_u32(&aux.o_done[t][(j & 1)]));
-        if (t == kTiles - 1) tc_commit_cta(smem_u32(&aux.v_empty[j & 1]));
+        if (t == used - 1) tc_commit_cta(smem_u32(&aux.v_empty[j & 1]));
       }
       __syncwarp();
     };
-    const bool second = kTiles == 2 && soft_warps(1) > 0;
     if (n_tiles > 0) {
       ok = mbar_wait_warp(smem_u32(&aux.q_full), 0, abort_flag, status, kStatusTileWait, lane) && wait(aux.k_full, 0);
       tc_fence_after();
@@ -339,11 +340,17 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const int blocks, const u
       tc_fence_after();
       values(0, j);
       if constexpr (kTiles == 2) {
-        if (second) ok = wait(aux.p_full[1], j);
+        if (used < 2) continue;
+        ok = wait(aux.p_full[1], j);
         if (!ok) break;
         tc_fence_after();
         values(1, j);
       }
+    }
+    // tensor memory and barriers are given up when every product has ended and its arrivals are there
+    for (int j = max(0, n_tiles - 2); j < n_tiles && ok; ++j) {
+      ok = wait(aux.k_empty, j) && wait(aux.v_empty, j);
+      for (int t = 0; t < used && ok; ++t) ok = wait(aux.o_done[t], j);
     }
   } else {
     // ---- softmax: a thread per row; the warp's quarter of tensor memory is its number modulo 4 ----
@@ -506,13 +513,13 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const int blocks, const u
 #pragma unroll
     for (int d = 0; d < D; d += 16) {
       uint32_t o[16];
-      if (n_tiles > 0) {
+      if (n_tiles > 0 && live) {
         tmem_ld16(o_at + d, o);
         tmem_ld_wait();
       }
       float x[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = none || n_tiles == 0 ? 0.f : __uint_as_float(o[i]) * by;
+      for (int i = 0; i < 16; ++i) x[i] = none || n_tiles == 0 || !live ? 0.f : __uint_as_float(o[i]) * by;
       if (mine && splits > 1) {
         float* dst = parts.acc + unit * D + d;
 #pragma unroll

@@ -613,3 +613,55 @@ def test_rows_of_unaligned_tensors(rows, dtype):
     q, out = wide[:, 3:3 + h * d], torch.zeros(2 * rows, h * d + 3, dtype=dtype, device=DEV)[:, 1:1 + h * d]
     run_prefix(q, cache, scales, tables, starts, lens, 0.1, out=out)
     check(out, attention_reference(q.reshape(-1, h, d), cache[0], cache[1], scales[0], scales[1], tables, starts, lens, 0.1), dtype)
+
+
+# ---- many rows --------------------------------------------------------------------------
+def attention_reference_by_request(q, k8, v8, ks, vs, tables, starts, lens, scale):
+    """`attention_reference` with all of a request's rows at a time."""
+    t, h, d = q.shape
+    bs, most = k8.shape[1], tables.shape[1] * k8.shape[1]
+    out, size, least = (torch.full((t, h, d), float("nan"), dtype=torch.double, device=DEV) for _ in range(3))
+    score, count = torch.zeros(t, h, 1, dtype=torch.double, device=DEV), torch.zeros(t, 1, 1, dtype=torch.double, device=DEV)
+    for r, n in enumerate(lens):
+        a, b = starts[r], starts[r + 1]
+        n = max(0, min(n, most))
+        if a == b:
+            continue
+        ids = tables[r, :-(-n // bs)].long()
+        k, v = ((c.view(torch.uint8)[ids].view(E4M3).double() * s[ids].double()[:, None, :, None]).flatten(0, 1)[:n].transpose(0, 1)
+                for c, s in ((k8, ks), (v8, vs)))                                                             # [H, n, D]
+        codes = v8.view(torch.uint8)[ids].view(E4M3).double().abs().flatten(0, 1)[:n].transpose(0, 1)
+        steps = vs[ids].double().repeat_interleave(bs, 0)[:n].transpose(0, 1)
+        x = q[a:b].double().transpose(0, 1)                                                                   # [H, rows, D]
+        keys = n - (b - 1 - torch.arange(a, b, device=DEV))
+        seen = torch.arange(n, device=DEV)[None, :] < keys[:, None]
+        p = torch.softmax((x @ k.transpose(1, 2) * scale).masked_fill(~seen, -float("inf")), dim=2).nan_to_num(0.0)
+        out[a:b], size[a:b] = (p @ v).transpose(0, 1), (p @ v.abs()).transpose(0, 1)
+        least[a:b] = (2.0 ** -32 * (p * steps[:, None]).amax(2, keepdim=True) * (seen.double() @ codes)).transpose(0, 1)
+        score[a:b, :, 0] = ((x.abs() @ k.abs().transpose(1, 2) * abs(scale)) * seen).amax(2).transpose(0, 1)
+        count[a:b, 0, 0] = keys.clamp_min(0).double()
+    return out, size, score, count, least
+
+
+def check_prefix(h, d, rows, lens, dtype, bs=16, scale=None):
+    nb, scale = sum(-(-n // bs) for n in lens) + 1, d ** -0.5 if scale is None else scale
+    cache, scales = make_cache(nb, bs, h, d, seed=d)
+    tables = make_tables(lens, bs, nb, seed=h)
+    spoil_behind(cache, tables, lens, bs)
+    starts = [0]
+    for n in rows:
+        starts.append(starts[-1] + n)
+    q = query(starts[-1], h, d, dtype)
+    got = run_prefix(q, cache, scales, tables, starts, lens, scale)
+    for _ in range(3):
+        assert torch.equal(got, run_prefix(q, cache, scales, tables, starts, lens, scale))
+    check(got, attention_reference_by_request(q.reshape(-1, h, d), cache[0], cache[1], scales[0], scales[1], tables, starts, lens, scale), dtype)
+    A.raise_on_device_status()
+
+
+@pytest.mark.parametrize("dtype", [F, B])
+@pytest.mark.parametrize("h,d", [(2, 64), (20, 64), (2, 128), (20, 128)])
+@pytest.mark.parametrize("rows,lens", [([520, 500], [700, 900]), ([257, 255, 200], [300, 256, 1100])])
+def test_pairs_of_row_tiles_of_which_the_second_is_empty(rows, lens, h, d, dtype):
+    """Two row tiles share a CTA; a request's last 1 ... 128 rows fill the first one alone.  Two heads: the tokens are cut into parts, too."""
+    check_prefix(h, d, rows, lens, dtype)
