@@ -156,7 +156,7 @@ kv8_combine_kernel(const Kv8Call c, const Kv8Parts a) {
     const float2 x = ml[i];
     const float w = exp2f(x.x - ref);
     sum = fmaf(w, x.y, sum);
-    s_w[i] = x.x == -INFINITY ? -1.f : w;   // a part without tokens has no acc
+    s_w[i] = x.x == -INFINITY ? -1.f : w;   // no acc: no tokens, or scores that are all NaN (0 times its sum is NaN then, too)
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
@@ -216,7 +216,10 @@ kv8_combine_few_kernel(const Kv8Call c, const Kv8Parts a) {
   for (int e = 0; e < kPer; ++e) x[e] = 0.f;
 #pragma unroll
   for (int i = 0; i < kFewParts; ++i) {
-    if (ml[i].x == -INFINITY) continue;   // a part without tokens has no acc
+    if (ml[i].x == -INFINITY) {   // no acc: a part without tokens, whose sum is 0, or one whose scores are all NaN, whose sum is NaN
+      sum += ml[i].y;
+      continue;
+    }
     const float w = exp2f(ml[i].x - ref);
     sum = fmaf(w, ml[i].y, sum);
 #pragma unroll

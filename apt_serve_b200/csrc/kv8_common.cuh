@@ -73,7 +73,8 @@ __device__ __forceinline__ float e4m3_scale(float top) {
 // Where the parts of rows whose tokens are cut go: [row][head][split], and the header of the scratch (PlanWord).
 struct Kv8Parts {
   int* plan;
-  float2* ml;                // maximum of the scores (log2) and sum of the weights relative to it; nothing attended: (-infinity, 0)
+  float2* ml;                // maximum of the scores (log2) and sum of the weights relative to it; nothing attended: (-infinity, 0), scores
+                             // that are all NaN: (-infinity, NaN)
   float* acc;                // weighted values, relative to that maximum
   int splits;                // 1: the output is written directly
   float scale_log2;

@@ -665,3 +665,22 @@ def check_prefix(h, d, rows, lens, dtype, bs=16, scale=None):
 def test_pairs_of_row_tiles_of_which_the_second_is_empty(rows, lens, h, d, dtype):
     """Two row tiles share a CTA; a request's last 1 ... 128 rows fill the first one alone.  Two heads: the tokens are cut into parts, too."""
     check_prefix(h, d, rows, lens, dtype)
+
+
+@pytest.mark.parametrize("tokens", [1000, 2048, 6000])
+@pytest.mark.parametrize("d,dtype,rows", [(64, F, 1), (128, B, 5), (64, B, 12), (128, F, 20), (64, F32, 2)])
+def test_a_whole_part_outside_the_cache_makes_its_rows_nan(d, dtype, rows, tokens):
+    """Tokens 512 ... 1023 are a part of their own, or several, in every kernel; two to eight parts, and more, are joined."""
+    bs, h, nb = 16, 2, -(-tokens // 16)
+    cache, scales = make_cache(nb, bs, h, d)
+    tables = make_tables([tokens], bs, nb)
+    q = query(rows, h, d, dtype)
+    want = run_prefix(q, cache, scales, tables, [0, rows], [tokens], 0.1)
+    assert not torch.isnan(want).any()
+    bad = tables.clone()
+    bad[0, 32:64] = nb
+    assert torch.isnan(run_prefix(q, cache, scales, bad, [0, rows], [tokens], 0.1)).all()
+    scales[0, tables[0, 32:64].long(), 0] = float("nan")
+    got = run_prefix(q, cache, scales, tables, [0, rows], [tokens], 0.1)
+    assert torch.isnan(got[:, :d]).all() and torch.equal(got[:, d:], want[:, d:])
+    A.raise_on_device_status()
