@@ -193,8 +193,8 @@ def paged_prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_c
     """Attention of several new tokens per request over its whole context in an 8-bit cache, the new tokens' own rows included (a chunk of
     a prompt behind a cached prefix, drafted tokens to be verified): rows ``query_start_loc[r] ... query_start_loc[r + 1]`` (int32
     ``[B + 1]``, at most ``max_query_len`` each) of ``query [T, H*D]`` are the last of request ``r``'s ``seq_lens[r]`` tokens, each
-    attends to the tokens up to itself -> ``[T, H*D]``.  Rows that belong to no request are left as they are in ``out``; rows of a request
-    beyond ``max_query_len`` are not computed."""
+    attends to the tokens up to itself -> ``[T, H*D]``.  Rows that belong to no request, and rows of a request
+    behind its first ``max_query_len``, are left as they are in ``out``."""
     return _attend_fp8("paged_prefix_attention", query, key_cache, value_cache, block_tables, query_start_loc, seq_lens, max_query_len,
                        scale, k_scale, v_scale, out, workspace)
 

@@ -24,7 +24,7 @@ struct Kv8Call {
   void* out; const void* query;
   Kv8Cache cache;
   const int32_t* tables; const int32_t* starts; const int32_t* seq_lens;
-  int batch, max_blocks, max_rows;   // max_rows: most rows of a request
+  int batch, max_blocks, max_rows;   // max_rows: most rows of a request; those of one that has more are left as they are
   int64_t rows, query_stride, out_stride;
   float scale;
   int dtype;
@@ -80,7 +80,8 @@ struct Kv8Parts {
   float scale_log2;
 };
 
-// The request of query row t, and how many tokens the row attends to (none: a zero row).  False: the row belongs to no request.
+// The request of query row t, and how many tokens the row attends to (none: a zero row).  False: the row belongs to no request, or
+// comes behind the max_rows first ones of its own.
 __device__ __forceinline__ bool kv8_find_row(const Kv8Call& c, int64_t t, int& req, int& keys) {
   if (c.starts == nullptr) {
     req = (int)t;
@@ -94,6 +95,7 @@ __device__ __forceinline__ bool kv8_find_row(const Kv8Call& c, int64_t t, int& r
     if (c.starts[mid] <= t) lo = mid; else hi = mid;
   }
   req = lo;
+  if (t - c.starts[req] >= c.max_rows) return false;
   const int ctx = max(0, min(c.seq_lens[req], c.max_blocks * c.cache.block_size));
   keys = max(0, ctx - c.starts[req + 1] + (int)t + 1);
   return true;

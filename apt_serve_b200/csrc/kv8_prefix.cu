@@ -127,8 +127,9 @@ __device__ __forceinline__ int longest_first(const Kv8Call& c, int blocks, int r
   __shared__ int s_tokens[kSorted], s_pair;
   for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
     const int req = i / blocks, row0 = (blocks - 1 - i % blocks) * kTall, n = c.starts[req + 1] - c.starts[req];
+    const int to = min(n, c.max_rows);
     const int ctx = max(0, min(c.seq_lens[req], c.max_blocks * c.cache.block_size));
-    s_tokens[i] = row0 < n ? max(0, ctx - n + min(n, row0 + kTall)) : -1;
+    s_tokens[i] = row0 < to ? max(0, ctx - n + min(to, row0 + kTall)) : -1;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
@@ -154,10 +155,11 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const int blocks, const u
   const int pair = longest_first<kTiles * kRows>(c, blocks, blockIdx.x / splits / c.cache.heads), req = pair / blocks;
   if (blockIdx.x == 0 && threadIdx.x == 0) parts.plan[kPlanStatus] = kStatusOk;
   const int start = c.starts[req], n_rows = c.starts[req + 1] - start, row0 = (blocks - 1 - pair % blocks) * (kTiles * kRows);
-  if (row0 >= n_rows) { chain_next(); return; }
+  const int rows_to = min(n_rows, c.max_rows);   // rows behind those are left as they are
+  if (row0 >= rows_to) { chain_next(); return; }
   const int bs = c.cache.block_size, ctx = max(0, min(c.seq_lens[req], c.max_blocks * bs));
   const int first = ctx - n_rows + row0;                                 // own position of the CTA's first row
-  const int rows_here = min(kTiles * kRows, n_rows - row0);
+  const int rows_here = min(kTiles * kRows, rows_to - row0);
   const int end = first + rows_here;                                     // tokens that its last row attends to, if any
   const int all_tiles = max(0, (end + kKeys - 1) / kKeys), per = (all_tiles + splits - 1) / splits;
   const int tile0 = min(all_tiles, split * per), n_tiles = min(all_tiles, tile0 + per) - tile0;

@@ -116,7 +116,7 @@ kv8_stream_kernel(const Kv8Call c, const Kv8Parts parts, const int part_groups, 
   const int head = blockIdx.x % c.cache.heads, part = blockIdx.x / c.cache.heads, req = part / parts.splits, split = part % parts.splits;
   if (blockIdx.x == 0 && threadIdx.x == 0) parts.plan[kPlanStatus] = kStatusOk;
   const int start = c.starts != nullptr ? c.starts[req] : req;
-  const int rows_all = c.starts != nullptr ? c.starts[req + 1] - start : 1, n_rows = min(kRows, rows_all);
+  const int rows_all = c.starts != nullptr ? c.starts[req + 1] - start : 1, n_rows = min(c.starts != nullptr ? min(kRows, c.max_rows) : 1, rows_all);
   if (n_rows <= 0) return;
   const int bs = c.cache.block_size, ctx = max(0, min(c.seq_lens[req], c.max_blocks * bs));
   const int first = ctx - rows_all;                    // own position of the first row

@@ -450,8 +450,8 @@ int aps_kv8_write(const void* key, const void* value, void* key_cache, void* val
  * Attention of query rows [num_rows, H, D] over that cache.  Row t belongs to the request r with query_start_loc[r] <= t <
  * query_start_loc[r + 1] (int32 [batch + 1]; NULL: one row per request, row r is request r's); a request's rows are the last of its
  * seq_lens[r] tokens, each attends to the tokens up to itself.  A row that attends to none (a length of 0, more rows than tokens) is
- * zero; rows before the first start and behind the last are left as they are.  max_query_len: no request has more rows (those of one
- * that has are not computed).  Scales of the cache are not negative.  A table entry outside [0, num_blocks) is not read: the rows that
+ * zero; rows before the first start and behind the last are left as they are.  max_query_len: no request has more rows (of one
+ * that has, those behind its first max_query_len are left as they are, too).  Scales of the cache are not negative.  A table entry outside [0, num_blocks) is not read: the rows that
  * attend to a token of it become NaN.  A NaN value row can also show in the rows of its request less than 256 before it.
  * fp16 and bf16 queries with head sizes 64 and 128 and a positive scale take tensor-core kernels, in which weights are rounded to fp16;
  * everything else is computed in fp32.

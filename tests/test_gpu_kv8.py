@@ -684,3 +684,22 @@ def test_a_whole_part_outside_the_cache_makes_its_rows_nan(d, dtype, rows, token
     got = run_prefix(q, cache, scales, tables, [0, rows], [tokens], 0.1)
     assert torch.isnan(got[:, :d]).all() and torch.equal(got[:, d:], want[:, d:])
     A.raise_on_device_status()
+
+
+@pytest.mark.parametrize("width", [None, 400])   # the latter's tokens are cut into more than eight parts
+@pytest.mark.parametrize("most", [0, 1, 5, 12, 20, 130, 300])
+@pytest.mark.parametrize("d,dtype", [(64, F), (128, B), (64, F32)])
+def test_rows_beyond_the_bound_of_a_requests_rows_are_left(d, dtype, most, width):
+    lens, rows, bs, h = [400, 350, 9], [310, 4, 9], 16, 2
+    cache, scales = make_cache(60, bs, h, d)
+    tables, seq = make_tables(lens, bs, 60, width=width), torch.tensor(lens, dtype=torch.int32, device=DEV)
+    starts = [0, 310, 314, 323]
+    q = query(323, h, d, dtype)
+    out = torch.full((323, h * d), 7.0, dtype=dtype, device=DEV)
+    A.paged_prefix_attention(q, cache[0], cache[1], tables, torch.tensor(starts, dtype=torch.int32, device=DEV), seq, most, 0.1, scales[0], scales[1],
+                             out=out)
+    within = torch.cat([torch.arange(n) < most for n in rows]).to(DEV)
+    assert (out[~within] == 7).all()
+    ref = attention_reference_by_request(q.reshape(-1, h, d), cache[0], cache[1], scales[0], scales[1], tables, starts, lens, 0.1)
+    check(out[within], tuple(x[within] for x in ref), dtype)
+    A.raise_on_device_status()
