@@ -504,8 +504,10 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const int blocks, const u
     ok = ok && (n_tiles == 0 || !live || wait(aux.o_done[tile], n_tiles - 1));
     tc_fence_after();
     const float bad = __int_as_float(0x7fc00000);
-    // O is relative to 2^(ref - kUp), the sum and the parts to 2^m
-    float by = ref == -INFINITY ? 0.f : ex2(ref - kUp - (m == -INFINITY ? 0.f : m));
+    // O is relative to 2^(ref - kUp), the sum and the parts to 2^m; in two steps, with the least scales the factor is 2^-133, below the
+    // normal range
+    const float root = ref == -INFINITY ? 0.f : ex2(0.5f * (ref - kUp - (m == -INFINITY ? 0.f : m)));
+    float by = root;
     const bool none = first + row < 0;    // a row before the first token
     const int64_t unit = (t * c.cache.heads + head) * splits + split;
     if (splits == 1) by /= l;             // nothing but scores of -infinity: NaN
@@ -521,7 +523,7 @@ kv8_tile_kernel(const Kv8Call c, const Kv8Parts parts, const int blocks, const u
       }
       float x[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = none || n_tiles == 0 || !live ? 0.f : __uint_as_float(o[i]) * by;
+      for (int i = 0; i < 16; ++i) x[i] = none || n_tiles == 0 || !live ? 0.f : __uint_as_float(o[i]) * root * by;
       if (mine && splits > 1) {
         float* dst = parts.acc + unit * D + d;
 #pragma unroll

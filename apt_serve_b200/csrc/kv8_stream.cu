@@ -334,13 +334,15 @@ kv8_stream_kernel(const Kv8Call c, const Kv8Parts parts, const int part_groups, 
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(kFull, sum, o);
       if (row >= n_rows || t < 0 || t >= c.rows) continue;
-      float by = ref[q][e] == -INFINITY ? 0.f : ex2(ref[q][e] - kUp - (m[q][e] == -INFINITY ? 0.f : m[q][e]));   // relative to 2^m
+      // relative to 2^m, in two steps: with the least scales the factor is 2^-133, below the normal range
+      const float root = ref[q][e] == -INFINITY ? 0.f : ex2(0.5f * (ref[q][e] - kUp - (m[q][e] == -INFINITY ? 0.f : m[q][e])));
+      float by = root;
       if (parts.splits == 1) by /= sum;    // nothing but scores of -infinity: NaN
       const bool none = first + row < 0;   // a row before the first token
       const int64_t unit = (t * c.cache.heads + head) * parts.splits + split;
       float x[kPer];
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) x[i] = none ? 0.f : acc[q][i / 2][2 * (i & 1) + e] * by;
+      for (int i = 0; i < kPer; ++i) x[i] = none ? 0.f : acc[q][i / 2][2 * (i & 1) + e] * root * by;
       if (parts.splits > 1) {
         float* dst = parts.acc + unit * D + kPer * g;
 #pragma unroll

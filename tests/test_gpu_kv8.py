@@ -703,3 +703,15 @@ def test_rows_beyond_the_bound_of_a_requests_rows_are_left(d, dtype, most, width
     ref = attention_reference_by_request(q.reshape(-1, h, d), cache[0], cache[1], scales[0], scales[1], tables, starts, lens, 0.1)
     check(out[within], tuple(x[within] for x in ref), dtype)
     A.raise_on_device_status()
+
+
+@pytest.mark.parametrize("d,dtype,rows", [(64, B, 1), (128, B, 7), (128, B, 12), (64, B, 60), (128, B, 200), (64, F32, 3)])
+def test_values_of_the_least_scale(d, dtype, rows):
+    """Outputs near 2^-112 are bf16 numbers like any other."""
+    lens, bs, h = [900], 16, 3
+    cache, scales = make_cache(60, bs, h, d)
+    tables = make_tables(lens, bs, 60)
+    scales[1] = 2.0 ** -118
+    q = query(rows, h, d, dtype)
+    ref = attention_reference_by_request(q.reshape(-1, h, d), cache[0], cache[1], scales[0], scales[1], tables, [0, rows], lens, 0.1)
+    check(run_prefix(q, cache, scales, tables, [0, rows], lens, 0.1), ref, dtype)
