@@ -69,7 +69,7 @@ PROTOTYPES = {
     "aps_kv8_write": (c_int, [c_void_p] * 7 + [c_int64] + [c_int] * 3 + [c_int64] * 5 + [c_void_p, c_size_t, c_int, c_void_p]),
     "aps_kv8_decode_step": (c_int, [c_void_p] * 9 + [c_int64] + [c_void_p] * 2 + [c_int] * 5 + [c_int64] * 7 +
                             [c_float, c_void_p, c_size_t, c_int, c_void_p]),
-    "aps_kv8_attention_workspace_bytes": (c_size_t, [c_int, c_int64] + [c_int] * 4),
+    "aps_kv8_attention_workspace_bytes": (c_size_t, [c_int, c_int64] + [c_int] * 6),
     "aps_kv8_attention": (c_int, [c_void_p] * 9 + [c_int, c_int64] + [c_int] * 5 + [c_int64] * 5 +
                           [c_float, c_void_p, c_size_t, c_int, c_void_p]),
     "aps_attention_status": (c_int, [c_void_p, c_void_p, c_void_p]),

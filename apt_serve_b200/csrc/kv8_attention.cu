@@ -8,6 +8,8 @@
 // Scores, softmax statistics and sums are fp32; a code times its scale is exact in fp32.
 #include "kv8_common.cuh"
 
+#include <initializer_list>
+
 namespace aps {
 namespace {
 
@@ -278,6 +280,9 @@ int launch_rows(const Kv8Call& c, const Kv8Parts& a, cudaStream_t stream) {
 
 enum Way { kRows, kStream, kTiles };
 
+Way way_of(const Kv8Call& c) { return kv8_stream_takes(c) ? kStream : kv8_tiles_take(c) ? kTiles : kRows; }
+int splits_of(const Kv8Call& c, Way way) { return way == kStream ? kv8_stream_splits(c) : way == kTiles ? kv8_tile_splits(c) : row_splits(c); }
+
 template <typename T>
 int attend(const Kv8Call& c, const Kv8Parts& a, Way way, cudaStream_t stream) {
   int st;
@@ -320,17 +325,23 @@ int check_call(const char* op, const Kv8Call& c) {
 
 using namespace aps;
 
-extern "C" size_t aps_kv8_attention_workspace_bytes(int batch, int64_t num_rows, int max_blocks_per_seq, int block_size, int num_heads, int head_size) {
-  if (batch <= 0 || num_rows <= 0 || max_blocks_per_seq <= 0 || block_size <= 0 || num_heads <= 0 || head_size <= 0) return 0;
+extern "C" size_t aps_kv8_attention_workspace_bytes(int batch, int64_t num_rows, int max_query_len, int max_blocks_per_seq, int block_size,
+                                                    int num_heads, int head_size, int dtype) {
+  if (batch <= 0 || num_rows <= 0 || max_query_len < 0 || max_blocks_per_seq <= 0 || block_size <= 0 || num_heads <= 0 || head_size <= 0) return 0;
   Kv8Call c{};
-  c.rows = num_rows; c.max_blocks = max_blocks_per_seq;
-  c.cache.heads = num_heads; c.cache.head_size = head_size; c.cache.block_size = block_size;
-  // the most that any of the kernels takes
-  c.batch = batch;
+  c.batch = batch; c.rows = num_rows; c.max_rows = max_query_len < num_rows ? max_query_len : (int)num_rows; c.max_blocks = max_blocks_per_seq;
+  c.cache.heads = num_heads; c.cache.head_size = head_size; c.cache.block_size = block_size; c.cache.num_blocks = 1;
+  c.scale = 1.f; c.dtype = dtype;
+  // what the kernel takes that such a call runs: with a scale that is not positive the CUDA-core one, with starts or (a row for each
+  // request) without
+  const int32_t some = 0;
   int most = row_splits(c);
-  if (kv8_stream_splits(c) > most) most = kv8_stream_splits(c);
-  for (int tiles = 1; tiles <= 2; ++tiles)
-    if (kv8_tile_splits(c, tiles) > most) most = kv8_tile_splits(c, tiles);
+  for (const int32_t* starts : {(const int32_t*)nullptr, &some}) {
+    if (starts == nullptr && num_rows != batch) continue;
+    c.starts = starts;
+    const int splits = splits_of(c, way_of(c));
+    most = splits > most ? splits : most;
+  }
   return part_scratch(num_rows, num_heads, head_size, most);
 }
 
@@ -343,8 +354,8 @@ int plan_attention(const Kv8Call& c, void* workspace, size_t workspace_bytes, Wa
   if (st != APS_OK || c.rows == 0 || c.batch == 0) return st;
   APS_REQUIRE(c.starts != nullptr || c.rows == c.batch, APS_ERR_SHAPE, "kv8_attention: %lld query rows for %d requests",
               (long long)c.rows, c.batch);
-  *way = kv8_stream_takes(c) ? kStream : kv8_tiles_take(c) ? kTiles : kRows;
-  const int splits = *way == kStream ? kv8_stream_splits(c) : *way == kTiles ? kv8_tile_splits(c) : row_splits(c);
+  *way = way_of(c);
+  const int splits = splits_of(c, *way);
   *a = Kv8Parts{static_cast<int*>(workspace), nullptr, nullptr, splits, c.scale * 1.4426950408889634f};
   const size_t need = part_scratch(c.rows, c.cache.heads, c.cache.head_size, splits);
   APS_REQUIRE(workspace != nullptr && aligned_to(workspace, 256) && workspace_bytes >= need, APS_ERR_WORKSPACE,

@@ -455,9 +455,10 @@ int aps_kv8_write(const void* key, const void* value, void* key_cache, void* val
  * attend to a token of it become NaN.  A NaN value row can also show in the rows of its request less than 256 before it.
  * fp16 and bf16 queries with head sizes 64 and 128 and a positive scale take tensor-core kernels, in which weights are rounded to fp16;
  * everything else is computed in fp32.
- * workspace: aps_kv8_attention_workspace_bytes(batch, num_rows, ...) bytes, 256-byte aligned; aps_attention_status reads its status word.
+ * workspace: aps_kv8_attention_workspace_bytes bytes of the call's own sizes, 256-byte aligned; aps_attention_status reads its status word.
  */
-size_t aps_kv8_attention_workspace_bytes(int batch, int64_t num_rows, int max_blocks_per_seq, int block_size, int num_heads, int head_size);
+size_t aps_kv8_attention_workspace_bytes(int batch, int64_t num_rows, int max_query_len, int max_blocks_per_seq, int block_size,
+                                         int num_heads, int head_size, int dtype);
 int aps_kv8_attention(void* out, const void* query, const void* key_cache, const void* value_cache, const float* key_scale,
                       const float* value_scale, const int32_t* block_tables, const int32_t* query_start_loc,
                       const int32_t* seq_lens, int batch, int64_t num_rows, int max_query_len, int max_blocks_per_seq,
@@ -467,7 +468,8 @@ int aps_kv8_attention(void* out, const void* query, const void* key_cache, const
 
 /*
  * The two for the decode tokens of a step, row r of key, value and query request r's: aps_kv8_write of num_slots rows, then
- * aps_kv8_attention of one row per request.  workspace: the larger of what the two take.
+ * aps_kv8_attention of one row per request.  workspace: the larger of what the two take
+ * (num_rows = batch, max_query_len = 1).
  */
 int aps_kv8_decode_step(void* out, const void* query, const void* key, const void* value, void* key_cache, void* value_cache,
                         float* key_scale, float* value_scale, const int64_t* slot_mapping, int64_t num_slots,

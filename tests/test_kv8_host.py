@@ -114,3 +114,21 @@ def test_cache_engine_moves_the_scales_with_the_blocks():
     assert CacheEngine.num_blocks_for_budget(10 * 16448, 2, 4, 64, 16, E4M3) == 10
     with pytest.raises(ValueError, match="shared cache"):
         CacheEngine(1, 4, 64, 16, 8, 4, E4M3, device="cpu", with_shared_cache=True, pin_memory=False)
+
+
+def test_scratch_is_that_of_the_kernel_that_runs():
+    """Parts of rows are held where the tokens are cut, which long chunks' are not: no row of theirs needs a place for each part that a
+    few rows would be cut into."""
+    def size(batch, rows, most, blocks, heads, d, dtype=torch.float16):
+        return N.lib().aps_kv8_attention_workspace_bytes(batch, rows, most, blocks, 16, heads, d, N.DTYPE_ENUM[dtype])
+    for dtype in (torch.float16, torch.bfloat16, torch.float32):
+        assert size(1, 2048, 2048, 1001, 32, 64, dtype) == size(1, 8192, 8192, 2048, 40, 128, dtype) == 256   # the header alone
+        for batch in (1, 2, 7, 60, 300):
+            for most in (17, 100, 129, 600, 5000):
+                # twice as many CTAs as SMs at most, 128 rows and heads' parts each
+                assert size(batch, batch * most, most, 2048, 12, 128, dtype) <= 256 * 2 + 2 * 148 * 128 * 130 * 4
+    # a few rows' parts: what the streaming kernel takes, for drafted tokens and for one row of each request
+    assert size(64, 320, 5, 128, 40, 128) == size(64, 320, 16, 128, 40, 128) > size(64, 320, 17, 128, 40, 128)
+    assert size(256, 256, 1, 128, 40, 128) == size(256, 256, 300, 128, 40, 128) < 32 << 20   # 300: without starts a row for each
+    assert size(256, 256, 1, 128, 12, 64, torch.float32) <= size(256, 256, 1, 128, 12, 64)
+    assert size(0, 5, 1, 4, 2, 64) == size(2, 0, 1, 4, 2, 64) == size(2, 5, -1, 4, 2, 64) == 0
