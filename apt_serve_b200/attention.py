@@ -200,7 +200,9 @@ def paged_prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_c
 
 
 @lru_cache(maxsize=256)
-def _fp8_scratch_bytes(batch: int, rows: int, max_rows: int, max_blocks: int, block_size: int, heads: int, head_size: int, dtype: int) -> int:
+def _fp8_scratch_bytes(device: int, batch: int, rows: int, max_rows: int, max_blocks: int, block_size: int, heads: int, head_size: int,
+                       dtype: int) -> int:
+    """On ``device``, which is the current one: the parts that rows are cut into are planned for its number of SMs."""
     return N.lib().aps_kv8_attention_workspace_bytes(batch, rows, max_rows, max_blocks, block_size, heads, head_size, dtype)
 
 
@@ -243,7 +245,7 @@ def _attend_fp8(op, query, key_cache, value_cache, block_tables, starts, seq_len
     dtype = N.dtype_enum(query)
     with N.on_device(dev):
         if workspace is None:
-            workspace, ws_bytes = _scratch_of(dev, _fp8_scratch_bytes(b, t, max_rows, tables[1], bs, h, d, dtype))
+            workspace, ws_bytes = _scratch_of(dev, _fp8_scratch_bytes(dev.index, b, t, max_rows, tables[1], bs, h, d, dtype))
         else:
             ws_bytes = workspace.numel() * workspace.element_size()
         N.check(N.lib().aps_kv8_attention(
@@ -912,7 +914,7 @@ class FlashAttentionImpl:
         out = torch.empty_like(query, memory_format=torch.contiguous_format)
         kc, ks, lib = kv_cache.data_ptr(), kv_scale.data_ptr(), N.lib()
         with N.on_device(dev):
-            ws, ws_bytes = _scratch_of(dev, _fp8_scratch_bytes(n, n, 1, table[1], cache[2], h, d, N.DTYPE_ENUM[dtype]))
+            ws, ws_bytes = _scratch_of(dev, _fp8_scratch_bytes(dev.index, n, n, 1, table[1], cache[2], h, d, N.DTYPE_ENUM[dtype]))
             N.check(lib.aps_kv8_decode_step(
                 out.data_ptr(), query.data_ptr(), key.data_ptr(), value.data_ptr(), kc, kc + planes[0], ks, ks + 4 * scale_steps[0],
                 slots.data_ptr(), n, tables.data_ptr(), lens.data_ptr(), n, table[1], h, d, cache[2], cache[1], q_steps[0], k_steps[0],

@@ -132,3 +132,19 @@ def test_scratch_is_that_of_the_kernel_that_runs():
     assert size(256, 256, 1, 128, 40, 128) == size(256, 256, 300, 128, 40, 128) < 32 << 20   # 300: without starts a row for each
     assert size(256, 256, 1, 128, 12, 64, torch.float32) <= size(256, 256, 1, 128, 12, 64)
     assert size(0, 5, 1, 4, 2, 64) == size(2, 0, 1, 4, 2, 64) == size(2, 5, -1, 4, 2, 64) == 0
+
+
+def test_scratch_sizes_are_kept_for_each_device(monkeypatch):
+    """They follow the current device's number of SMs."""
+    class Lib:
+        sms = 148
+
+        def aps_kv8_attention_workspace_bytes(self, *sizes):
+            return self.sms * 1000
+    lib = Lib()
+    monkeypatch.setattr(N, "lib", lambda: lib)
+    sizes = (3, 3, 1, 4001, 16, 3, 64, 1)
+    first = A._fp8_scratch_bytes(0, *sizes)
+    lib.sms = 160
+    assert A._fp8_scratch_bytes(1, *sizes) == 160000 and A._fp8_scratch_bytes(0, *sizes) == first == 148000
+    A._fp8_scratch_bytes.cache_clear()
