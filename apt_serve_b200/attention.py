@@ -33,6 +33,8 @@ from .metadata import derive_private_block_tables
 # scratch
 # ----------------------------------------------------------------------------- #
 _workspaces: Dict[torch.device, torch.Tensor] = {}
+_captured: Dict[torch.device, torch.Tensor] = {}   # the scratch that calls have been captured with last
+_outgrown: List[torch.Tensor] = []                 # graphs work in it, later calls need more
 
 
 def _workspace(device: torch.device, need: int) -> torch.Tensor:
@@ -44,13 +46,18 @@ def _workspace(device: torch.device, need: int) -> torch.Tensor:
 
 
 def _scratch_of(device: torch.device, need: int) -> Tuple[torch.Tensor, int]:
-    """The per-device scratch tensor, and how many of its bytes a call that asks for ``need`` is given."""
+    """The per-device scratch tensor, and how many of its bytes a call that asks for ``need`` is given.  One that a captured call works
+    in is kept when a later call needs more: the graph's replays write to it."""
     need = max(need, 1 << 20)
     ws = _workspaces.get(device)
     if ws is None or ws.numel() < need:
+        if ws is not None and ws is _captured.get(device):
+            _outgrown.append(ws)
         ws = torch.empty(need, dtype=torch.uint8, device=device)
         ws[:256].zero_()   # no call has left a status in it
         _workspaces[device] = ws
+    if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+        _captured[device] = ws
     return ws, need
 
 

@@ -715,3 +715,26 @@ def test_values_of_the_least_scale(d, dtype, rows):
     q = query(rows, h, d, dtype)
     ref = attention_reference_by_request(q.reshape(-1, h, d), cache[0], cache[1], scales[0], scales[1], tables, [0, rows], lens, 0.1)
     check(run_prefix(q, cache, scales, tables, [0, rows], lens, 0.1), ref, dtype)
+
+
+def test_a_captured_call_keeps_its_scratch_when_a_later_one_needs_more(monkeypatch):
+    monkeypatch.setattr(A, "_workspaces", {})
+    lens, bs, h, d = [9000], 16, 4, 128
+    cache, scales = make_cache(563, bs, h, d)
+    tables, seq, q = make_tables(lens, bs, 563), torch.tensor(lens, dtype=torch.int32, device=DEV), query(1, h, d, F)
+
+    def attend(n=1):
+        return A.paged_decode_attention(q.repeat(n, 1), cache[0], cache[1], tables.repeat(n, 1), seq.repeat(n), 0.1,
+                                        k_scale=scales[0], v_scale=scales[1])
+    want = attend()
+    size = A._workspaces[q.device].numel()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = attend()
+    attend(64)
+    assert A._workspaces[q.device].numel() > size
+    torch.cuda.synchronize()
+    others = [torch.zeros(size, dtype=torch.uint8, device=DEV) for _ in range(4)]   # what the allocator has free of that size
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and not any(x.any() for x in others)

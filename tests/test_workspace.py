@@ -34,3 +34,31 @@ def test_scratch_of_a_few_requests_is_small():
     assert size(8, 39, torch.float16) < 2 * one and size(256, 128, torch.float16) > 10 * one
     small = N.lib().aps_decode_layer_step_workspace_bytes(1, 39, 16, 12, 64, 768, N.DTYPE_ENUM[torch.float32])
     assert small < 4 << 20
+
+
+def test_scratch_of_captured_calls_is_kept(monkeypatch):
+    """A graph goes on working in it after a call that needs more."""
+    monkeypatch.setattr(A, "_workspaces", {})
+    monkeypatch.setattr(A, "_captured", {})
+    monkeypatch.setattr(A, "_outgrown", [])
+    capturing = [False]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    empty = torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *a, device, **kw: empty(*a, **kw))
+    device = torch.device("cuda", 0)
+    A._scratch_of(device, 2 << 20)
+    A._scratch_of(device, 3 << 20)
+    assert A._outgrown == []      # no graph knew it
+    capturing[0] = True
+    first = A._scratch_of(device, 1 << 20)[0]
+    assert first.numel() == 3 << 20
+    capturing[0] = False
+    assert A._scratch_of(device, 2 << 20)[0] is first
+    second = A._scratch_of(device, 4 << 20)[0]
+    third = A._scratch_of(device, 5 << 20)[0]
+    assert len(A._outgrown) == 1 and A._outgrown[0] is first and third is not second
+    capturing[0] = True
+    fourth = A._scratch_of(device, 6 << 20)[0]   # allocated under capture
+    capturing[0] = False
+    A._scratch_of(device, 7 << 20)
+    assert len(A._outgrown) == 2 and A._outgrown[1] is fourth
