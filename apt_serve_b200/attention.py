@@ -787,7 +787,7 @@ class FlashAttentionImpl:
         fp32 ``[2, NB, H]``, which the writes set (``ops.reshape_and_cache_flash``); hidden-cached requests are refused."""
         if self.fp8_cache:
             return self._forward_fp8(query, key, value, kv_cache, attn_metadata, kv_scale)
-        assert not isinstance(kv_scale, torch.Tensor) and kv_scale == 1.0, "kv_scale is not supported in FlashAttention."
+        assert (not isinstance(kv_scale, torch.Tensor) or kv_scale.numel() == 1) and kv_scale == 1.0, "kv_scale is not supported in FlashAttention."
         if attn_metadata.num_prefill_tokens == 0 and attn_metadata.num_hidden_cache_tokens == 0:
             output = self._plain_decode(query, key, value, kv_cache, attn_metadata)
             if output is not None:

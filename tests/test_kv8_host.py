@@ -148,3 +148,17 @@ def test_scratch_sizes_are_kept_for_each_device(monkeypatch):
     lib.sms = 160
     assert A._fp8_scratch_bytes(1, *sizes) == 160000 and A._fp8_scratch_bytes(0, *sizes) == first == 148000
     A._fp8_scratch_bytes.cache_clear()
+
+
+def test_a_16_bit_cache_takes_the_number_one_as_a_scale():
+    """As a tensor, too; not the scales of an 8-bit cache."""
+    class Meta:
+        num_hidden_cache_tokens = num_decode_tokens = num_prefill_tokens = num_prefills = num_tot_tokens = 0
+        block_tables = seq_lens_tensor = prefill_metadata = decode_metadata = None
+        slot_mapping = torch.zeros(0, dtype=torch.int64)
+    x, impl = torch.zeros(0, 128), A.FlashAttentionImpl(2, 64, 1.0, 2, None, None, "auto")
+    for one in (1.0, 1, torch.tensor(1.0), torch.ones(1)):
+        assert impl.forward(x, x, x, None, None, Meta, one).shape == (0, 128)
+    for other in (0.5, torch.tensor(2.0), torch.ones(2, 4, 2)):
+        with pytest.raises(AssertionError, match="kv_scale"):
+            impl.forward(x, x, x, None, None, Meta, other)
