@@ -24,6 +24,14 @@ constexpr int kThreads = 256;
 
 __device__ int g_kv8_status = 0;   // a slot past the cache has been met since this was read last
 
+// Whether there has been a write on the current device (of which a captured one may be replayed at any time): reading the status is a
+// copy to the host, which callers without an 8-bit cache are spared.
+bool* written_here() {
+  static bool written[64] = {false};
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 ? &written[dev] : nullptr;
+}
+
 struct WriteArgs {
   const void *key, *value;
   uint8_t *key_cache, *value_cache;
@@ -467,6 +475,11 @@ int write_by_head(const WriteArgs& a, int head_size, bool aligned, void* ws, cud
 }  // namespace
 
 int read_kv8_status(int* host_status, cudaStream_t stream) {
+  const bool* written = written_here();
+  if (written != nullptr && !*written) {
+    *host_status = 0;
+    return APS_OK;
+  }
   void* addr = nullptr;
   APS_CUDA(cudaGetSymbolAddress(&addr, g_kv8_status));
   APS_CUDA(cudaMemcpyAsync(host_status, addr, sizeof(int), cudaMemcpyDeviceToHost, stream));
@@ -521,6 +534,7 @@ extern "C" int aps_kv8_write(const void* key, const void* value, void* key_cache
   const size_t need = write_scratch(num_tokens, num_blocks);
   APS_REQUIRE(need == 0 || (workspace != nullptr && aligned_to(workspace, 256) && workspace_bytes >= need), APS_ERR_WORKSPACE,
               "kv8_write: workspace must be 256-byte aligned and hold %zu bytes (got %zu)", need, workspace_bytes);
+  if (bool* written = written_here()) *written = true;
   const bool aligned = aligned_to(key, 16) && aligned_to(value, 16) && key_stride * es % 16 == 0 && value_stride * es % 16 == 0 &&
                        aligned_to(key_cache, 8) && aligned_to(value_cache, 8) && block_stride % 8 == 0;
   const WriteArgs a{key, value, (uint8_t*)key_cache, (uint8_t*)value_cache, key_scale, value_scale, slot_mapping, num_tokens,

@@ -9,6 +9,10 @@ and 2^-25 for fp16 outputs below the normal range.  A weight times its block's v
 one below 2^-14, fp16's normal range, is off by 2^-25 instead, so the output by
     2^-25 2^-7 max_t (p_t s_t) sum_t |code_t|
 more, which shows where the tokens that have the weight have next to nothing in a dimension."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -738,3 +742,31 @@ def test_a_captured_call_keeps_its_scratch_when_a_later_one_needs_more(monkeypat
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want) and not any(x.any() for x in others)
+
+
+_STATUS = """
+import torch
+from torch.profiler import ProfilerActivity, profile
+from apt_serve_b200 import attention as A, ops
+dev = torch.device("cuda", 0)
+
+def copies():
+    with profile(activities=[ProfilerActivity.CUDA]) as p:
+        A.cache_ops_status(dev)
+    return sum(e.name.startswith("Memcpy DtoH") for e in p.events())
+x, slots = torch.zeros(2, 2, 64, device=dev, dtype=torch.float16), torch.tensor([3, 99], device=dev)
+A.cache_ops_status(dev)
+before = copies()
+cache, scales = torch.zeros(2, 4, 16, 2, 64, device=dev, dtype=torch.float8_e4m3fn), torch.zeros(2, 4, 2, device=dev)
+ops.reshape_and_cache_flash(x, x, cache[0], cache[1], slots, "fp8", scales[0], scales[1])
+assert A.cache_ops_status(dev) == 2 and A.cache_ops_status(dev) == 0
+print("copies", before, copies())
+"""
+
+
+def test_reading_the_status_costs_no_more_where_no_8_bit_cache_is_written():
+    """Every word of the status is a copy to the host that is waited for."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", _STATUS], cwd=root, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout
+    assert "copies 3 4" in r.stdout, r.stdout
