@@ -770,3 +770,37 @@ def test_reading_the_status_costs_no_more_where_no_8_bit_cache_is_written():
     r = subprocess.run([sys.executable, "-c", _STATUS], cwd=root, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=300)
     assert r.returncode == 0, r.stdout
     assert "copies 3 4" in r.stdout, r.stdout
+
+
+@pytest.mark.parametrize("dtype", [F, B])
+@pytest.mark.parametrize("h,d,rows,lens", [
+    (2, 64, [1000], [3000]), (20, 128, [700, 690, 650], [700, 2000, 651]),   # several pairs of row tiles a request
+    (1, 64, [129 + r % 7 for r in range(260)], [140 + r % 50 for r in range(260)]),   # more pairs than are put in order
+    (1, 128, [17 + r % 3 for r in range(300)], [30 + r % 90 for r in range(300)]),    # as many single tiles
+])
+def test_prefix_of_many_rows_and_requests(h, d, rows, lens, dtype):
+    check_prefix(h, d, rows, lens, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, F, B])
+@pytest.mark.parametrize("h,d,bs", [(3, 64, 16), (2, 128, 32), (1, 256, 16), (5, 32, 16)])
+def test_a_decode_step_in_one_call(h, d, bs, dtype):
+    """Ragged requests, one that begins a block, one of a single token, one longer than a part; several steps."""
+    lens, nb = [40, 33, 1, 700, 16], 60
+    cache, scales = make_cache(nb, bs, h, d, seed=6)
+    impl = A.FlashAttentionImpl(h, d, 0.11, h, None, None, "fp8")
+    tables = make_tables([n + 3 for n in lens], bs, nb)
+    for step in range(3):
+        now = [n + step for n in lens]
+        slots = torch.tensor([int(tables[r, (n - 1) // bs]) * bs + (n - 1) % bs for r, n in enumerate(now)], device=DEV)
+        q, (k, v) = query(5, h, d, dtype, seed=step), rows_of(5, h, d, dtype, seed=step)
+        want = [(cache[p].cpu().view(torch.uint8).clone(), scales[p].cpu().clone()) for p in (0, 1)]
+        for p, rows in ((0, k), (1, v)):
+            write_reference(*want[p], rows.cpu(), slots.tolist(), bs)
+        meta = metadata(None, now, tables, slots, None)
+        got = impl._plain_decode_fp8(q, k.reshape(5, -1), v.reshape(5, -1), cache, meta, scales)
+        assert got is not None
+        for p in (0, 1):
+            assert same_codes(cache[p], want[p][0]) and torch.equal(scales[p].cpu(), want[p][1])
+        check(got, attention_reference(q.reshape(-1, h, d), cache[0], cache[1], scales[0], scales[1], tables, list(range(6)), now, 0.11), dtype)
+    A.raise_on_device_status()
