@@ -12,7 +12,7 @@
 //   many rows   runs of neighbouring rows in neighbouring slots of one block are listed first (prompts are nothing else), with how many
 //               such runs a block has; a block that has one is done from its run, others by looking through the mapping
 // What bounds it: bytes, (element size + 1) for each element of prompts' rows; launch and three round trips for single tokens.  24 OPT-13B
-// prompts in fp16 (592 MB) 135 us, 67 % of the measured copy rate: 32 warps per SM with 4 KB each in flight, half of the issue slots.
+// prompts in fp16 (592 MB) 126 us, 72 % of the measured copy rate: 32 warps per SM with 4 KB each in flight, half of the issue slots.
 #include "kv8_common.cuh"
 
 #include <type_traits>
@@ -247,8 +247,9 @@ __device__ __forceinline__ bool write_rows(const WriteArgs& a, int plane, int he
 
 // For what almost all blocks get: up to 16 rows, 16 bytes at a time, all of them in registers; no infinities, a scale that is a power of
 // two, no other rows to be rounded to it.  False: nothing has been written, one of the forms above has to do it (after the kernel's other
-// heads: between them its registers would be this one's; in one function with the form above 24 OPT-13B prompts took 158 us, so 125).
-template <typename T, int D, bool kAligned>
+// heads: between them its registers would be this one's; in one function with the form above 24 OPT-13B prompts took 158 us, so 126).
+// Offset: of a row in the block; 32 bits where the block has 16 rows (with 64, and one call for both forms, they took 135).
+template <typename T, int D, bool kAligned, typename Offset>
 __device__ __forceinline__ bool write_head(const WriteArgs& a, int plane, int head, const BlockRows& b, int lane) {
   using C = RowCfg<T, D>;
   using P = Pack<T, C::kPer>;
@@ -278,7 +279,7 @@ __device__ __forceinline__ bool write_head(const WriteArgs& a, int plane, int he
   const float need = e4m3_scale(top), s = anew ? need : fmaxf(old, need), by = 1.f / s;
   if (!(top <= 3.402823466e38f) || (__float_as_uint(s) & 0x7fffffu) != 0 || (!anew && s != old)) return false;
   uint8_t* held = (plane ? a.value_cache : a.key_cache) + (int64_t)b.block * a.block_stride + (int64_t)head * D + column;
-  const int64_t held_row = (int64_t)a.heads * D;
+  const Offset held_row = (Offset)a.heads * D;
   const bool in_half = std::is_same<T, __half>::value && by >= 6.103515625e-05f && by <= 32768.f;
 #pragma unroll
   for (int i = 0; i < C::kLoads; ++i) {
@@ -353,7 +354,7 @@ kv8_write_kernel(const WriteArgs a) {
   if (u >= 2 * a.heads) return;
   const int plane = u >= a.heads, head = plane ? u - a.heads : u;
   const BlockRows b{block, s_n, 0, 0, slots, token};
-  if (!write_head<T, D, kAligned>(a, plane, head, b, lane) && !write_rows<T, D, kAligned>(a, plane, head, b, lane))
+  if (!write_head<T, D, kAligned, int64_t>(a, plane, head, b, lane) && !write_rows<T, D, kAligned>(a, plane, head, b, lane))
     write_any_head<T, D>(a, plane, head, b, lane);
 }
 
@@ -401,10 +402,13 @@ kv8_write_runs_kernel(const WriteArgs a, const Runs r) {
       const int2 after = run_at(k + 2), next_info = r.blocks[block_of(then)];
       const uint32_t block = block_of(now);
       const int from = now.y - (int)(block * (uint32_t)a.block_size);
-      const BlockRows b{block, info.y - now.x + 1, now.x, from, nullptr, nullptr};
-      bool done = info.x == 1;
-      if (done) done = kShort ? write_head<T, D, kAligned>(a, plane, head, b, lane) : write_rows<T, D, kAligned>(a, plane, head, b, lane);
-      if (!done) left |= 1u << k;
+      if constexpr (kShort) {
+        if (info.x != 1 || !write_head<T, D, kAligned, int>(a, plane, head, BlockRows{block, info.y - now.x + 1, now.x, from, nullptr, nullptr}, lane))
+          left |= 1u << k;
+      } else {
+        if (info.x != 1 || !write_rows<T, D, kAligned>(a, plane, head, BlockRows{block, info.y - now.x + 1, now.x, from, nullptr, nullptr}, lane))
+          left |= 1u << k;
+      }
       now = then; then = after; info = next_info;
     }
     for (; left != 0; left &= left - 1) {
