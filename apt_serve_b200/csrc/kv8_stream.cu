@@ -89,15 +89,16 @@ __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
 // tables of up to 16 groups are not cut and parts have eight at least.  Where parts of up to 40 fill the GPU once, as many as fill it
 // (a 30 011-token OPT-1.3B context: 26 groups 34 us, 16 37, 48 41); else 16, and 32 where there are many of them (128 OPT-66B tp 8
 // requests: 16 groups 69 us, 32 77; 256 OPT-13B requests 519 and 500).
-constexpr int64_t kUnits = 148 * 16;   // warps on the GPU at a time
+int64_t units_at_once() { return (int64_t)sm_count() * 16; }   // warps on the GPU at a time (the kernel of 9 - 16 rows: 10 an SM, not planned for)
 int part_groups(const Kv8Call& c) {
+  const int64_t gpu = units_at_once();
   const int64_t each = (int64_t)c.max_blocks * c.cache.block_size / 16, units = (int64_t)c.batch * c.cache.heads;
   if (each <= 16) return 16;
-  if (units < kUnits) {
-    const int64_t parts = kUnits / units, n = (each + parts - 1) / parts;
+  if (units < gpu) {
+    const int64_t parts = gpu / units, n = (each + parts - 1) / parts;
     if (n <= 40) return (int)(n < 8 ? 8 : n);
   }
-  return each * units < 128 * kUnits ? 16 : 32;
+  return each * units < 128 * gpu ? 16 : 32;
 }
 
 template <int D> __host__ __device__ constexpr int stages() { return D == 128 ? 3 : 6; }   // groups of a warp in shared memory
@@ -409,7 +410,7 @@ bool kv8_stream_takes(const Kv8Call& c) {
 int kv8_stream_splits(const Kv8Call& c) {
   const int64_t groups = (int64_t)c.max_blocks * c.cache.block_size / 16, n = (groups + part_groups(c) - 1) / part_groups(c);
   // with many units and wide tables (of which the lengths may use little) no more than a few
-  const int64_t units = (int64_t)c.batch * c.cache.heads, most = (kUnits * 4 + units - 1) / units;
+  const int64_t units = (int64_t)c.batch * c.cache.heads, most = (units_at_once() * 4 + units - 1) / units;
   const int64_t some = n < most ? n : most < 4 ? (n < 4 ? n : 4) : most;
   return (int)(some > 1024 ? 1024 : some);   // as many as the joining kernel takes
 }
