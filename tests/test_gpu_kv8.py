@@ -629,7 +629,9 @@ def attention_reference_by_request(q, k8, v8, ks, vs, tables, starts, lens, scal
     for r, n in enumerate(lens):
         a, b = starts[r], starts[r + 1]
         n = max(0, min(n, most))
-        if a == b:
+        if n == 0:
+            out[a:b] = size[a:b] = least[a:b] = 0.0
+        if a == b or n == 0:
             continue
         ids = tables[r, :-(-n // bs)].long()
         k, v = ((c.view(torch.uint8)[ids].view(E4M3).double() * s[ids].double()[:, None, :, None]).flatten(0, 1)[:n].transpose(0, 1)
