@@ -11,16 +11,22 @@
 // scores (log2), for the sum of the weights l, and R, the maximum of score + log2(value scale), for the weights that meet V: so a block
 // of small values that has all the weight fills fp16's range like any other.  O stays in tensor memory and is rescaled only when R has
 // grown by more than 2^8.  The output is O 2^(R - m) / l.
+// The weights go into P V as one fp16 term.  Prompts' own attention (prefill_attention.cu) adds the rounded rest as a second one, because
+// its rows are exact and the weights' 2^-11 shows in its outputs; here every row has been rounded to 4 bits, 2.6e-2 of it, beside which
+// outputs at 2.8e-4 of those over the codes, where 2.1e-4 are the rounding of fp16 outputs (bf16 1.66e-3 and 1.65e-3), show next to nothing.
+// The second term would double P V's instructions and took a fifth of the time there.
 // bf16 queries become fp16 with a power of two for each row, which leaves 2^-40 of the row's largest element.
 //
-// Measured on one B200: 500 new tokens each of six OPT-13B requests behind 1500 (83 GFLOP) 177 us, 2048 of a 16 001-token OPT-1.3B document
-// (251 GFLOP) 514.  A pair of row tiles takes 1900 cycles a key tile (D = 64; 128: 2400) where its exponentials take 1024 (16 a cycle and SM), the products
-// 640 (D = 64) to 1280: a softmax warp is busy for 1700 of them, 1100 in the exponentials, which both tiles take at the same time; issue
-// slots 46 %, special function unit 56 %.  Tried, chunks / document, us: key tiles of 128 with one S 270 / 785 (183 / 517 without, before the
-// copies were tile by tile); beside 185 / 528: the second row tile held back by half a turn 196 / 563, two threads per row 200 / 569, a
-// quarter of the exponentials as polynomials 194 / 578, three stages of K and V 191 / 544, one row tile per CTA for long requests too 205 /
-// 561; a warp for the products of each row tile, with and without that half turn, 180 - 184 / 523; with D = 64 the queries in tensor memory
-// 515 (514 from shared memory).
+// Measured on one B200: 500 new tokens each of six OPT-13B requests behind 1000 (83 GFLOP) 178 us, 2048 of a 16 001-token OPT-1.3B document
+// (251 GFLOP) 514 (bf16 183 and 516).  A pair of row tiles takes 1900 cycles a key tile (D = 64; 128: 2400) where its exponentials take
+// 1024 (16 a cycle and SM), the products 640 (D = 64) to 1280: a softmax warp is busy for 1700 of them, 1100 in the exponentials, which
+// both tiles take at the same time; issue slots 46 %, special function unit 57 % (document; chunks 32 and 29 %).
+// Registers: two CTAs an SM leave the one-tile form 96, of which 48 - 52 bytes are spilled, in bf16 with D = 128 448; the two-tile form
+// spills 52 bytes there and none elsewhere.
+// Tried, chunks / document, us: key tiles of 128 with one S 270 / 785 (183 / 517 without, before the copies were tile by tile); beside
+// 185 / 528: the second row tile held back by half a turn 196 / 563, two threads per row 200 / 569, a quarter of the exponentials as
+// polynomials 194 / 578, three stages of K and V 191 / 544, one row tile per CTA for long requests too 205 / 561; a warp for the products
+// of each row tile, with and without that half turn, 180 - 184 / 523; with D = 64 the queries in tensor memory 515 (514 from shared memory).
 #include "kv8_common.cuh"
 #include "sm100.cuh"
 

@@ -11,7 +11,8 @@
 //   O^T += V^T P^T  A (16 dims x 16 tokens): tokens 2 j, 2 j + 1, 2 j + 8, 2 j + 9 of the lane's D / 8 consecutive dims, the tokens
 //                 paired by a byte permutation; tile i has dims (D / 8) g + 2 i and + 1 in rows g and g + 8.  P^T comes from S^T's
 //                 layout by a transposition in registers (movmatrix)
-// Every e4m3 number is an fp16 number.  The scales and the weights' two references are those of the tile kernel (kv8_prefix.cu).
+// Every e4m3 number is an fp16 number.  The scales, the weights' two references and their one fp16 term are those of the tile kernel
+// (kv8_prefix.cu).
 // Measured on one B200: one row of 256 OPT-13B requests (2.69 GB) 501 us back to back, 82 % of the measured copy rate.  What bounds it is
 // half memory and half the warps' own instructions (about 210 a group of 16 tokens: 64 conversions and 16 permutations, 16 products, 50
 // for the softmax).  Before this form: registers as the only staging 904 us, a ring of asynchronous copies 573, the query rows as the

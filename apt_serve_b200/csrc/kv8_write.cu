@@ -11,8 +11,12 @@
 //   few rows    every row's CTAs look through the whole mapping; those of a block's first row do the block (one launch)
 //   many rows   runs of neighbouring rows in neighbouring slots of one block are listed first (prompts are nothing else), with how many
 //               such runs a block has; a block that has one is done from its run, others by looking through the mapping
-// What bounds it: bytes, (element size + 1) for each element of prompts' rows; launch and three round trips for single tokens.  24 OPT-13B
-// prompts in fp16 (592 MB) 126 us, 72 % of the measured copy rate: 32 warps per SM with 4 KB each in flight, half of the issue slots.
+// What bounds it: bytes, (element size + 1) for each element of prompts' rows; launch and three round trips (mapping; scale and
+// rows; the block's other rows) for few single tokens, rounds of CTAs that each look through the mapping for many: 256 tokens of 40 x 128
+// are 2560 CTAs, 592 at a time, 15 us.  24 OPT-13B prompts in fp16 (592 MB) 126 us, 72 % of the measured copy rate: the loads' latency at
+// the 32 warps an SM that registers leave room for, 4 KB each in flight (47 % of its warps, 53 % of the issue slots).
+// Spills, at 64 registers: rows of 128 in the kernels for runs 84 - 88 bytes, with blocks of more than 16 rows 208 - 224; rows of 256 up to
+// 728; fp32, at 128 registers, 4 - 88.
 #include "kv8_common.cuh"
 
 #include <type_traits>
